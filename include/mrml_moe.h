@@ -65,6 +65,8 @@ typedef enum {
  * mrml_moe_prepare_weights (no counterpart in the reference). */
 enum { MRML_Q4_0 = 2, MRML_Q8_0 = 8, MRML_PACKED = 0x100 };
 enum { MRML_Q4_0_PACKED = MRML_Q4_0 | MRML_PACKED, MRML_Q8_0_PACKED = MRML_Q8_0 | MRML_PACKED };
+/* Element types of the permutation and MXFP4 operators (GGML ids too). */
+enum { MRML_F32 = 0, MRML_F16 = 1, MRML_BF16 = 30 };
 
 /* Library version (major*10000 + minor*100 + patch). */
 int mrml_moe_version(void);
@@ -369,6 +371,116 @@ int mrml_moe_geglu(const float *gate, const float *up, float *out, size_t n, mrm
  * n is a multiple of 32; dst holds n/32*34 (Q8_0) or n/32*18 (Q4_0) bytes. */
 int mrml_moe_quantize_q8_0(const float *src, uint8_t *dst, size_t n, mrml_stream_t stream);
 int mrml_moe_quantize_q4_0(const float *src, uint8_t *dst, size_t n, mrml_stream_t stream);
+
+/* ---- Tokens sorted by expert and back, with gradients. --------------------
+ * No counterpart in the reference, whose MoE re-reads the experts per
+ * (token, slot).  For experts of the caller's own: sort the pairs, gather
+ * the tokens' rows, run the experts on contiguous rows, bring the rows back.
+ * Row type `type` is MRML_F32, MRML_F16 or MRML_BF16; sums run in f32, in
+ * slot order, and are rounded once; results do not vary between calls.
+ * ld* are row strides in elements (at least H); the sorted rows are
+ * contiguous.  Rows whose addresses and strides are multiples of 16 bytes
+ * move in 16-byte vectors, others element by element. */
+
+/* Rows of the sorted order, an upper bound with each expert's rows padded to
+ * a multiple of `align` (1..128): T*K + min(E, T*K) * (align - 1); negative
+ * (MRML_ERR_INVALID_ARGUMENT) for invalid arguments. */
+int mrml_moe_sorted_rows(int E, int K, int T, int align);
+
+/* Counting sort of the pairs p = t*K + k by ids[p], stable: expert e's pairs
+ * take rows offsets[e] ... offsets[e] + counts[e] - 1 in pair order, every
+ * offset a multiple of `align`.  offsets has E + 1 entries (the last: the
+ * rows in use), counts E, pos T*K (the pair's row, or -1), pair
+ * mrml_moe_sorted_rows(E, K, T, align) (the row's pair, or -1 for padding and
+ * past the end).  A negative id marks a slot without an expert; an id of E or
+ * more is skipped too and sets MRML_ERR_BAD_EXPERT_ID in the workspace
+ * (mrml_moe_device_status).  E <= 256, K <= 64.  Workspace: clear it once
+ * with mrml_moe_workspace_init. */
+size_t mrml_moe_sort_workspace_bytes(int E, int K, int T);
+int mrml_moe_sort(const int32_t *ids, int32_t *offsets, int32_t *counts, int32_t *pos, int32_t *pair, int E, int K,
+                  int T, int align, void *workspace, size_t workspace_bytes, mrml_stream_t stream);
+
+/* rows[r] = x[pair[r] / K], zero where pair[r] is -1, for all n_rows rows. */
+int mrml_moe_permute(int type, const void *x, int64_t ldx, const int32_t *pair, void *rows, int H, int K, int n_rows,
+                     mrml_stream_t stream);
+
+/* Its gradient: dx[t] = sum_k drows[pos[t,k]] over the slots with a row. */
+int mrml_moe_permute_grad(int type, const void *drows, const int32_t *pos, void *dx, int64_t lddx, int H, int K, int T,
+                          mrml_stream_t stream);
+
+/* out[t] = sum_k probs[t,k] * rows[pos[t,k]] over the slots with a row (0 for
+ * a token with none); probs NULL means weights of 1. */
+int mrml_moe_unpermute(int type, const void *rows, const int32_t *pos, const float *probs, void *out, int64_t ldo,
+                       int H, int K, int T, mrml_stream_t stream);
+
+/* Its gradients: drows[pos[t,k]] = probs[t,k] * dout[t] (rows without a pair
+ * are zeroed, all n_rows >= T*K of them) and dprobs[t,k] = <dout[t],
+ * rows[pos[t,k]]> (0 for a slot without a row).  Either output may be NULL;
+ * rows is read for dprobs only. */
+int mrml_moe_unpermute_grad(int type, const void *dout, int64_t lddout, const void *rows, const int32_t *pos,
+                            const int32_t *pair, const float *probs, void *drows, float *dprobs, int H, int K, int T,
+                            int n_rows, mrml_stream_t stream);
+
+/* ---- MXFP4: microscaled 4-bit floating point. ------------------------------
+ * Blocks of 32 values along the summed axis share a power-of-two scale 2^e,
+ * e = max(floor(log2(max |v|)) - 2, -127); values are E2M1 (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 and a sign) times the scale, rounded to nearest, ties to even,
+ * saturating at 6.  (The rule of the Open Compute Project's Microscaling
+ * Formats 1.0.)  A block with an infinity or a NaN becomes NaN.  The last
+ * block of a row may be short.  No counterpart in the reference (GGUF Q4_0
+ * and Q8_0 only); results are those of MXFP4, not the reference's.
+ *
+ * A quantised matrix is opaque: mrml_moe_mx4_bytes bytes, 16-byte aligned, in
+ * the order in which the tensor cores' operands lie in shared memory (17/32
+ * byte per value, rows padded to 128 and columns to 64). */
+size_t mrml_moe_mx4_bytes(int rows, int cols, int matrices);
+
+/* Quantises `matrices` matrices of rows x cols (row stride ldx, matrix stride
+ * matrix_stride, both in elements; matrix_stride is ignored for one matrix).
+ * type: MRML_F32, MRML_F16, MRML_BF16, or MRML_Q4_0 / MRML_Q8_0 for
+ * contiguous GGUF blocks (cols a multiple of 32, ldx = cols, matrix_stride =
+ * rows * cols).  gated != 0: the rows are I gate rows then I up rows of a
+ * GeGLU (rows = 2I), laid out for mrml_moe_mx4_experts. */
+int mrml_moe_mx4_quantize(int type, const void *x, int64_t ldx, int64_t matrix_stride, uint8_t *dst, int rows,
+                          int cols, int matrices, int gated, mrml_stream_t stream);
+
+/* One read, both directions: dst is x [rows][cols] quantised along its rows,
+ * dst_t its transpose [cols][rows] quantised along x's columns, for the
+ * products of a training step: y = x w^T, dx = dy w, dw = dy^T x are
+ * mrml_moe_mx4_matmul of (x, w), (dy, w^T) and (dy^T, x^T). */
+int mrml_moe_mx4_quantize_both(int type, const void *x, int64_t ldx, uint8_t *dst, uint8_t *dst_t, int rows, int cols,
+                               mrml_stream_t stream);
+
+/* The values a quantised matrix stands for (type MRML_F32, MRML_F16 or
+ * MRML_BF16; f32 and bf16 hold every value that f32 and bf16 inputs give
+ * exactly). */
+int mrml_moe_mx4_dequantize(int type, const uint8_t *src, void *out, int64_t ldo, int64_t matrix_stride, int rows,
+                            int cols, int matrices, int gated, mrml_stream_t stream);
+
+/* out[M][N] = a [M][K] times b [N][K] transposed, both quantised (gated = 0),
+ * summed in f32 on the tensor cores and rounded once to `type`.  Workspace
+ * as above (its status word reports a bounded wait that gave up). */
+size_t mrml_moe_mx4_matmul_workspace_bytes(int M, int N, int K);
+int mrml_moe_mx4_matmul(int type, const uint8_t *a, const uint8_t *b, void *out, int64_t ldo, int M, int N, int K,
+                        void *workspace, size_t workspace_bytes, mrml_stream_t stream);
+
+/* A linear layer: x [T][K] of `type` quantised, then the product with w
+ * [N][K] (quantised). */
+size_t mrml_moe_mx4_linear_workspace_bytes(int T, int N, int K);
+int mrml_moe_mx4_linear(int type, const void *x, int64_t ldx, const uint8_t *w, void *out, int64_t ldo, int T, int N,
+                        int K, void *workspace, size_t workspace_bytes, mrml_stream_t stream);
+
+/* The experts and the combine in MXFP4 (mrml_moe_experts' place in a layer):
+ *   out[t] = sum_k probs[t,k] down_scale[e] down_e(Q(gelu_tanh(gate_e Q(x_t)) * up_e Q(x_t))),  e = ids[t,k],
+ * Q the quantisation above, everything else in f32.  gate_up: E matrices of
+ * 2I x H, quantised with gated = 1; down: E matrices of H x I.  down_scale
+ * may be NULL (1.0).  Slots with a negative id are left out (no threshold on
+ * probs); an id of E or more is left out and reported by
+ * mrml_moe_device_status.  Any H, I >= 1, E <= 256, K <= 64. */
+size_t mrml_moe_mx4_experts_workspace_bytes(int H, int I, int E, int K, int T);
+int mrml_moe_mx4_experts(int type, const uint8_t *gate_up, const uint8_t *down, const int32_t *ids, const float *probs,
+                         const float *down_scale, const void *x, int64_t ldx, void *out, int64_t ldo, int H, int I,
+                         int E, int K, int T, void *workspace, size_t workspace_bytes, mrml_stream_t stream);
 
 /* Process-wide options.  MRML_OPTION_EXPERT_PATH selects how the expert
  * products run: 0 automatic (the pipelined kernel with warp-level MMA from 2

@@ -197,6 +197,39 @@ cudaError_t launch_ep_combine_push(uint8_t* const* slabs, int rank, int N, int T
                                    const float* down_scale, cudaStream_t s);
 cudaError_t launch_ep_reduce(uint8_t* const* slabs, int rank, int N, int T, int H, int E, int K, const int32_t* ids,
                              const float* probs, float* out, int* err, cudaStream_t s);
+// (token, slot) pairs sorted by expert, rows gathered and brought back
+// (permute.cu).  sort_chunk_ints: ints of scratch for large sorts.
+size_t sort_chunk_ints(long long n_pairs, int E);
+cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, int32_t* pos, int32_t* pair, int E,
+                        int n_pairs, int align, int n_rows, int32_t* chunk_cnt, int* err, cudaStream_t s);
+cudaError_t launch_permute(int type, const void* x, long long ldx, const int32_t* pair, void* rows, int H, int K,
+                           int n_rows, cudaStream_t s);
+cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, const float* probs, void* out,
+                             long long ldo, int H, int K, int T, cudaStream_t s);
+// The same from f32 rows, with the weights times scale[ids] (scale may be null).
+cudaError_t launch_unpermute_f32(int type, const float* rows, const int32_t* pos, const float* probs,
+                                 const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                 cudaStream_t s);
+cudaError_t launch_unpermute_grad(int type, const void* dout, long long ldd, const void* rows, const int32_t* pos,
+                                  const int32_t* pair, const float* probs, void* drows, float* dprobs, int H, int K,
+                                  int T, int n_rows, cudaStream_t s);
+
+// MXFP4 matrices (mx4.cu, mx4_gemm.cu; layout in mx4.cuh).
+cudaError_t launch_mx4_quantize(int type, const void* x, long long ldx, long long mstride, uint8_t* dst, int rows,
+                                int cols, int matrices, bool gated, cudaStream_t s);
+cudaError_t launch_mx4_quantize_both(int type, const void* x, long long ldx, uint8_t* dst, uint8_t* dst_t, int rows,
+                                     int cols, cudaStream_t s);
+cudaError_t launch_mx4_dequantize(int type, const uint8_t* src, void* out, long long ldo, long long mstride, int rows,
+                                  int cols, int matrices, bool gated, cudaStream_t s);
+cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int32_t* pos, uint8_t* dst, int T, int H,
+                              int K, cudaStream_t s);
+// Token rows x (times) weight rows w.  With offsets / counts: E weight
+// matrices, each for its expert's token rows (which start at multiples of
+// 128); without: one matrix and n_tokens rows.  gated: the weights are in the
+// gated row order and the MXFP4 result act = gelu(gate) * up replaces out.
+cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
+                            const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
+                            long long ldo, uint8_t* act, long long max_token_tiles, int* err, cudaStream_t s);
 int gate_up_tok_chunk(int wtype, int H);
 int down_tok_chunk(int wtype, int I);
 

@@ -39,20 +39,44 @@ void record_event(cudaEvent_t e, cudaStream_t s) {
     cudaEventRecord(e, s);
 }
 
-struct LaunchMark {
-  cudaStream_t s;
-  explicit LaunchMark(cudaStream_t st) : s(st) {
-    if (t_events && t_next_event + 1 < t_n_events) record_event(t_events[t_next_event], s);
-  }
-  ~LaunchMark() {
-    if (t_events && t_next_event + 1 < t_n_events) {
-      record_event(t_events[t_next_event + 1], s);
-      t_next_event += 2;
-    }
-  }
-};
+}  // namespace
 
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+namespace mrml {
+
+LaunchMark::LaunchMark(cudaStream_t st) : s(st) {
+  if (t_events && t_next_event + 1 < t_n_events) record_event(t_events[t_next_event], s);
+}
+LaunchMark::~LaunchMark() {
+  if (t_events && t_next_event + 1 < t_n_events) {
+    record_event(t_events[t_next_event + 1], s);
+    t_next_event += 2;
+  }
+}
+
+// Once per device: is it an sm_100 part?
+int check_device() {
+  static std::atomic<int> verdict[mrml::kMaxDevices];  // 0 unknown, 1 ok, -1 wrong arch
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MRML_ERR_CUDA;
+  int v = dev >= 0 && dev < mrml::kMaxDevices ? verdict[dev].load(std::memory_order_relaxed) : 0;
+  if (v == 0) {
+    int major = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return MRML_ERR_CUDA;
+    v = major == 10 ? 1 : -1;
+    if (dev >= 0 && dev < mrml::kMaxDevices) verdict[dev].store(v, std::memory_order_relaxed);
+  }
+  return v == 1 ? MRML_OK : MRML_ERR_DEVICE;
+}
+
+}  // namespace mrml
+
+namespace {
+
+using mrml::LaunchMark;
+using mrml::align256;
+using mrml::aligned16;
+using mrml::check_device;
+using mrml::cuda_status;
 
 // Largest token tile of the tensor-core path; position buffers carry this
 // much slack so that a tile starting at the last position stays in bounds.
@@ -208,31 +232,6 @@ SideStream* side_stream() {
   return &ss;
 }
 
-// Once per device: is it an sm_100 part?
-int check_device() {
-  static std::atomic<int> verdict[mrml::kMaxDevices];  // 0 unknown, 1 ok, -1 wrong arch
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MRML_ERR_CUDA;
-  int v = dev >= 0 && dev < mrml::kMaxDevices ? verdict[dev].load(std::memory_order_relaxed) : 0;
-  if (v == 0) {
-    int major = 0;
-    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return MRML_ERR_CUDA;
-    v = major == 10 ? 1 : -1;
-    if (dev >= 0 && dev < mrml::kMaxDevices) verdict[dev].store(v, std::memory_order_relaxed);
-  }
-  return v == 1 ? MRML_OK : MRML_ERR_DEVICE;
-}
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-int cuda_status(cudaError_t e) { return e == cudaSuccess ? MRML_OK : MRML_ERR_CUDA; }
-
-#define MRML_TRY(expr)                 \
-  do {                                 \
-    const int _st = (expr);            \
-    if (_st != MRML_OK) return _st;    \
-  } while (0)
-
 // Weight type without the packed-layout flag, and the flag.
 int base_type(int wtype) { return wtype & ~MRML_PACKED; }
 bool is_packed(int wtype) { return (wtype & MRML_PACKED) != 0; }
@@ -266,12 +265,6 @@ int check_workspace(void* ws, size_t ws_bytes, int H, int I, int E, int K, int T
   if (ws_bytes < carve(nullptr, H, I, E, K, T).bytes) return MRML_ERR_WORKSPACE_TOO_SMALL;
   return MRML_OK;
 }
-
-#define MRML_LAUNCH(expr)              \
-  do {                                 \
-    LaunchMark _mark(s);               \
-    MRML_TRY(cuda_status(expr));       \
-  } while (0)
 
 // The L2 prefetch of mrml_moe_forward: the first experts' gate/up slabs
 // (the decode kernel's first wave of work units reads the experts in id

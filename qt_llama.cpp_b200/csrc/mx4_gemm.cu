@@ -1,0 +1,403 @@
+// mx4_gemm.cu — products of MXFP4 matrices on the 5th-generation tensor cores.
+//
+//   out[t][n] = sum_b 2^(ea[t,b] + eb[n,b]) sum_i a[t,32b+i] w[n,32b+i]
+//
+// tcgen05.mma kind::mxf4 multiplies E2M1 codes, applies both blocks' scales
+// and accumulates in f32 in tensor memory: a product of two codes is exact,
+// and so is its scaling, so the only roundings are the f32 additions.
+//
+// The weights are the instruction's A operand (128 rows, the only M of one
+// CTA for this kind) and the tokens its B operand (N = the tokens of the tile
+// rounded up to 16), so a decode step with a handful of tokens per expert
+// wastes tensor time (which it has) instead of memory traffic (which bounds
+// it), and the same kernel serves prompts with N = 128.
+//
+// A work unit is (expert, 128 weight rows, 128 token rows).  One persistent
+// CTA per SM takes units in turn:
+//   warp 0     producer: one bulk copy per operand and K chunk (the matrix
+//              format is the shared-memory operand layout, mx4.cuh)
+//   warp 1     TMEM allocation; lane 0 copies the chunk's scales to tensor
+//              memory and issues the MMAs
+//   warps 4-7  epilogue, on the other of two accumulators
+// Scales live in tensor memory per shared-memory stage, so a stage's scales
+// are overwritten only after the MMAs that read them have completed.
+// Every wait is bounded; on a timeout the CTA records the error, drains its
+// copies and MMAs (bounded again), frees its TMEM and returns.
+#include "../../include/mrml_moe.h"
+#include "kernels.h"
+#include "mx4.cuh"
+#include "pipe.cuh"
+
+namespace mrml {
+namespace mx {
+
+using tc::fence_after;
+using tc::fence_before;
+using tc::mbar_arrive;
+using tc::mma_commit;
+using tc::tmem_wait_ld;
+using tc::wait_bar;
+
+constexpr int kStages = 5;
+constexpr int kStageBytes = 2 * kMxChunkBytes;
+constexpr int kThreads = 256;
+constexpr int kExPitch = 65;                        // f32 per row of the GeGLU exchange
+constexpr int kExBytes = kMxRows * kExPitch * 4;    // 128 rows x 64 tokens
+constexpr uint32_t kAcc0 = 0, kAccCols = 128;       // two accumulators of 128 columns
+constexpr uint32_t kSf0 = 256, kSfCols = 16;        // scales: 8 + 8 columns per stage
+
+struct Params {
+  const uint8_t* w;        // weight tiles [E][w_tiles]
+  const uint8_t* x;        // token tiles
+  const int32_t* offsets;  // [E + 1] first token row per expert, multiples of 128; null: one matrix of n_tokens rows
+  const int32_t* counts;   // [E] tokens per expert
+  int E, n_tokens, w_tiles, nb;
+  int n_out;               // outputs per token: weight rows, or I for the gated product
+  void* out;               // [token row][ldo]
+  long long ldo;
+  uint8_t* act;            // gated: MXFP4 [token row][n_out]
+  int* err;
+};
+
+struct __align__(8) Bars {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem_base;
+  int abort;
+  int first[kMaxExperts + 1];  // token tiles of earlier experts
+};
+static_assert(sizeof(Bars) <= 2048, "the barrier block must fit its part of shared memory");
+constexpr int kBarBytes = 2048;
+
+// Shared-memory operand descriptor, K-major without swizzle: core matrices of
+// 8 rows x 16 bytes, 128 bytes apart along K and `sbo` along the rows.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46;
+}
+
+// Instruction descriptor of kind::mxf4: E2M1 operands (1), both K-major, E8M0
+// scales (bit 23), M = 128; N in bits 17-22 (N / 8), the scales' pair within
+// their 32-bit column in bits 4-5 (B) and 29-30 (A).
+__device__ __forceinline__ uint32_t idesc(int N, int sf) {
+  return (uint32_t)sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | 1u << 23 | (uint32_t)(kMxRows >> 4) << 24 |
+         (uint32_t)sf << 29;
+}
+
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb,
+                                         bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"((uint32_t)add));
+}
+
+// 32 lanes x 16 bytes of shared memory to four TMEM columns, the same in each
+// of the four lane quarters.
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t addr) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(addr, 128)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Whether `ok` holds in all 128 threads of the epilogue (a barrier of theirs).
+__device__ __forceinline__ bool all_epilogue(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
+}
+
+// A unit: its expert, weight tile, first token row and tokens.
+struct Unit {
+  int wt, row0, n;
+  size_t w_tile;
+};
+
+__device__ __forceinline__ Unit unit_of(const Params& P, const Bars* B, int u) {
+  Unit U;
+  int e = 0, t;
+  if (P.offsets) {
+    // expert: the last with first[e] * w_tiles <= u
+    const int tile = u / P.w_tiles;  // token tile index over all experts, up to the order inside an expert
+    int lo = 0, hi = P.E;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (B->first[mid] <= tile) lo = mid;
+      else hi = mid;
+    }
+    e = lo;
+    const int tt = B->first[e + 1] - B->first[e], r = u - B->first[e] * P.w_tiles;
+    U.wt = r / tt;
+    t = r % tt;
+    U.row0 = P.offsets[e] + t * kMxRows;
+    U.n = min(kMxRows, P.counts[e] - t * kMxRows);
+  } else {
+    const int tt = (P.n_tokens + kMxRows - 1) / kMxRows;
+    U.wt = u / tt;
+    t = u % tt;
+    U.row0 = t * kMxRows;
+    U.n = min(kMxRows, P.n_tokens - U.row0);
+  }
+  U.w_tile = (size_t)e * P.w_tiles + U.wt;
+  return U;
+}
+
+// gelu_tanh(g) * u; 0.5 g (1 + tanh(z)) = g / (1 + exp(-2z)), which keeps its
+// relative precision for large negative g.  The exponent saturates harmlessly:
+// exp -> inf gives 0, exp -> 0 gives g.
+__device__ __forceinline__ float geglu(float g, float u) {
+  const float z2 = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+  return __fdividef(g, 1.f + __expf(-z2)) * u;
+}
+
+enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Bars* B = reinterpret_cast<Bars*>(smem_raw);
+  uint8_t* ring = smem_raw + kBarBytes;
+  float* ex = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // GeGLU exchange
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&B->full[i], 1);
+      mbar_init(&B->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->acc_full[i], 1);
+      mbar_init(&B->acc_empty[i], 4);
+    }
+    mbar_init(&B->drain, 1);
+    B->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem_base)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (P.offsets && warp == 2) {  // token tiles before each expert
+    constexpr int kPer = kMaxExperts / 32;
+    int c[kPer], s = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int x = lane * kPer + i;
+      c[i] = s;
+      if (x < P.E) s += (P.counts[x] + kMxRows - 1) / kMxRows;
+    }
+    int up = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += y;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane * kPer + i < P.E) B->first[lane * kPer + i] = up - s + c[i];
+    if (lane == 31) B->first[P.E] = up;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = B->tmem_base;
+  const int n_units = (P.offsets ? B->first[P.E] : (P.n_tokens + kMxRows - 1) / kMxRows) * P.w_tiles;
+  const int nc = (P.nb + kMxChunk - 1) / kMxChunk;
+  const size_t tile_bytes = mx_tile_bytes(P.nb);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
+        const Unit U = unit_of(P, B, u);
+        const uint8_t* wsrc = P.w + U.w_tile * tile_bytes;
+        const uint8_t* xsrc = P.x + (size_t)(U.row0 / kMxRows) * tile_bytes;
+        const int groups = ((U.n + 15) & ~15) >> 3;
+        for (int c = 0; c < nc; ++c) {
+          if (!(ok = wait_bar(&B->empty[s], ph ^ 1, B, P.err))) break;
+          const int n = min(kMxChunk, P.nb - c * kMxChunk);
+          const uint32_t wb = mx_chunk_bytes(n), xb = mx_scale_bytes(n) + groups * n * 128;
+          uint8_t* dst = ring + s * kStageBytes;
+          mbar_arrive_expect_tx(&B->full[s], wb + xb);
+          bulk_g2s(dst, wsrc + (size_t)c * kMxChunkBytes, wb, &B->full[s]);
+          bulk_g2s(dst + kMxChunkBytes, xsrc + (size_t)c * kMxChunkBytes, xb, &B->full[s]);
+          ++issued;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // Whatever happened, every copy lands before the block gives up its
+      // shared memory.
+      for (int i = 0; i < min(issued, kStages); ++i) {
+        if (--s < 0) {
+          s = kStages - 1;
+          ph ^= 1;
+        }
+        mbar_wait_bounded(&B->full[s], ph, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0, a = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
+        const Unit U = unit_of(P, B, u);
+        const int N = (U.n + 15) & ~15;
+        if (!(ok = wait_bar(&B->acc_empty[a], aph ^ 1, B, P.err))) break;
+        fence_after();
+        const uint32_t acc = tmem + kAcc0 + a * kAccCols;
+        for (int c = 0; c < nc; ++c) {
+          if (!(ok = wait_bar(&B->full[s], ph, B, P.err))) break;
+          fence_after();
+          const int n = min(kMxChunk, P.nb - c * kMxChunk);
+          const uint32_t wa = smem_u32(ring + s * kStageBytes), xa = wa + kMxChunkBytes;
+          const uint32_t sf = tmem + kSf0 + s * kSfCols, sb = mx_scale_bytes(n);
+          for (uint32_t g = 0; g < sb; g += 512) {
+            copy_scales(sf + g / 128, wa + g);
+            copy_scales(sf + 8 + g / 128, xa + g);
+          }
+          for (int j = 0; j < n / 2; ++j)
+            mma_mxf4(acc, desc(wa + sb + j * 256, n * 128), desc(xa + sb + j * 256, n * 128), idesc(N, (j & 1) * 2),
+                     sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, c + j > 0);
+          mma_commit(&B->empty[s]);
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        mma_commit(&B->acc_full[a]);
+        if (a ^= 1; a == 0) aph ^= 1;
+      }
+      mma_commit(&B->drain);  // and every MMA ends before the TMEM goes
+      mbar_wait_bounded(&B->drain, 0, nullptr);
+    }
+  } else if (warp >= 4) {
+    const int q = warp & 3;
+    int a = 0;
+    uint32_t aph = 0;
+    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
+      const Unit U = unit_of(P, B, u);
+      bool ok = wait_bar(&B->acc_full[a], aph, B, P.err);
+      // All lanes leave together; all four warps where they meet at barriers.
+      if constexpr (MODE == kModeGated) ok = all_epilogue(ok);
+      else ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + kAcc0 + a * kAccCols;
+      uint32_t r[32];
+      if constexpr (MODE == kModeGated) {
+        // 64 tokens at a time: all rows to shared memory (rows 0..63 gate,
+        // 64..127 up), then a thread per (token, block of 32 outputs).
+        const int tid = threadIdx.x - 128;
+        const int nba = mx_blocks(P.n_out);
+        for (int c0 = 0; c0 < U.n; c0 += 64) {
+#pragma unroll
+          for (int h = 0; h < 64; h += 32) {
+            if (c0 + h >= U.n) break;
+            tmem_ld32(acc + c0 + h, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ex[(32 * q + lane) * kExPitch + h + i] = __uint_as_float(r[i]);
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const int t = tid & 63, b = tid >> 6;
+          const int row = U.row0 + c0 + t, blk = U.wt * 2 + b;
+          if (c0 + t < U.n && blk < nba) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[i] = geglu(ex[(32 * b + i) * kExPitch + t], ex[(64 + 32 * b + i) * kExPitch + t]);
+            uint4 codes;
+            const uint32_t s = mx_quantize32(v, codes);
+            uint8_t* tile = P.act + (size_t)(row / kMxRows) * mx_tile_bytes(nba);
+            *reinterpret_cast<uint4*>(tile + mx_code_offset(nba, row % kMxRows, blk)) = codes;
+            tile[mx_scale_offset(row % kMxRows, blk)] = (uint8_t)s;
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+      } else {
+        using E = Elem<MODE == kModeF32 ? kF32 : MODE == kModeF16 ? kF16 : kBF16>;
+        const int f = U.wt * kMxRows + 32 * q + lane;
+        typename E::T* out = static_cast<typename E::T*>(P.out) + (long long)U.row0 * P.ldo + f;
+        for (int c0 = 0; c0 < U.n; c0 += 32) {
+          tmem_ld32(acc + c0, r);
+          tmem_wait_ld();
+          if (f < P.n_out) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c0 + i < U.n) out[(long long)(c0 + i) * P.ldo] = E::put(__uint_as_float(r[i]));
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B->acc_empty[a]);
+      if (a ^= 1; a == 0) aph ^= 1;
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+template <int MODE>
+cudaError_t launch(const Params& P, int units, cudaStream_t s) {
+  static SmemOptIn cache;
+  const size_t smem = kBarBytes + kStages * kStageBytes + (MODE == kModeGated ? kExBytes : 0);
+  const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE>, smem, cache);
+  if (st != cudaSuccess) return st;
+  return launch_pdl(mx4_gemm_kernel<MODE>, dim3(std::max(1, std::min(units, tc_num_sms()))), dim3(kThreads), smem, s, P);
+}
+
+}  // namespace mx
+
+cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
+                            const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
+                            long long ldo, uint8_t* act, long long max_token_tiles, int* err, cudaStream_t s) {
+  mx::Params P{};
+  P.w = w;
+  P.x = x;
+  P.offsets = offsets;
+  P.counts = counts;
+  P.E = E;
+  P.n_tokens = n_tokens;
+  P.w_tiles = (rows + kMxRows - 1) / kMxRows;
+  P.nb = mx_blocks(cols);
+  P.n_out = gated ? rows / 2 : rows;
+  P.out = out;
+  P.ldo = ldo;
+  P.act = act;
+  P.err = err;
+  const int units = (int)std::min<long long>(max_token_tiles * P.w_tiles, 1 << 20);
+  if (gated) return mx::launch<mx::kModeGated>(P, units, s);
+  switch (type) {
+    case kF32: return mx::launch<mx::kModeF32>(P, units, s);
+    case kF16: return mx::launch<mx::kModeF16>(P, units, s);
+    default: return mx::launch<mx::kModeBF16>(P, units, s);
+  }
+}
+
+}  // namespace mrml

@@ -1,0 +1,411 @@
+// permute.cu — (token, slot) pairs sorted by expert, the tokens' rows gathered
+// in that order and brought back with weights, and the gradients of both.
+//
+//   sort       pos[p] = offsets[e] + #{q < p : ids[q] = e} for e = ids[p]
+//   permute    rows[r] = x[pair[r] / K]
+//   its gradient and unpermute
+//              out[t] = sum_k w[t,k] rows[pos[t,k]]   (w = 1 for the gradient)
+//   unpermute's gradients
+//              drows[pos[t,k]] = w[t,k] dout[t],  dw[t,k] = <dout[t], rows[pos[t,k]]>
+// Sums run in f32 in slot order and are rounded once.
+#include "../../include/mrml_moe.h"
+#include "kernels.h"
+#include "mx4.cuh"
+
+namespace mrml {
+
+namespace {
+
+// -------------------------------------------------------------------- sort
+// Counting sort, stable by construction: a warp owns consecutive pairs, ranks
+// those of one expert with a warp match, and starts from the counts of the
+// warps (and chunks) before it.  No atomic decides an order.
+struct SortArgs {
+  const int32_t* ids;
+  int32_t *offsets, *counts, *pos, *pair;
+  int32_t* chunk_cnt;  // [chunks][E], more than one chunk only
+  int* err;
+  int n_pairs, E, align, n_rows, chunk;
+};
+
+__global__ void __launch_bounds__(1024) sort_count_kernel(SortArgs a) {
+  __shared__ int cnt[kMaxExperts];
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) cnt[e] = 0;
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  const int p0 = blockIdx.x * a.chunk, p1 = min(a.n_pairs, p0 + a.chunk);
+  for (int p = p0 + threadIdx.x; p < p1; p += blockDim.x) {
+    const int e = a.ids[p];
+    if ((unsigned)e < (unsigned)a.E) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.chunk_cnt[(size_t)blockIdx.x * a.E + e] = cnt[e];
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
+  extern __shared__ int sm[];
+  const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = a.E;
+  int* wcnt = sm;              // [nw][E] pairs of this chunk's earlier warps
+  int* tot = wcnt + nw * E;    // [E] pairs of all chunks
+  int* before = tot + E;       // [E] pairs of earlier chunks
+  int* off = before + E;       // [E + 1]
+  for (int i = threadIdx.x; i < nw * E + 2 * E; i += blockDim.x) sm[i] = 0;
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  int e[ITEMS], rank[ITEMS];
+  const int p0 = blockIdx.x * a.chunk + warp * 32 * ITEMS;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int p = p0 + i * 32 + lane;
+    e[i] = p < a.n_pairs ? a.ids[p] : -1;
+    if (e[i] >= E) {
+      set_error(a.err, kDevBadExpert);
+      e[i] = -1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+    const int at = __popc(same & ((1u << lane) - 1));
+    if (e[i] >= 0) rank[i] = wcnt[warp * E + e[i]] + at;
+    __syncwarp();
+    if (e[i] >= 0 && at == 0) wcnt[warp * E + e[i]] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < E; x += blockDim.x) {
+    int s = 0;
+    for (int w = 0; w < nw; ++w) {
+      const int c = wcnt[w * E + x];
+      wcnt[w * E + x] = s;
+      s += c;
+    }
+    if (gridDim.x == 1) tot[x] = s;
+  }
+  if (gridDim.x > 1) {
+    // this chunk's start and the totals, from every chunk's counts
+    for (int i = threadIdx.x; i < (int)gridDim.x * E; i += blockDim.x) {
+      const int c = a.chunk_cnt[i], x = i % E;
+      if (c) {
+        atomicAdd(&tot[x], c);
+        if (i / E < (int)blockIdx.x) atomicAdd(&before[x], c);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // aligned starts: each lane scans E / 32 experts
+    constexpr int kPer = kMaxExperts / 32;
+    int c[kPer], s = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int x = lane * kPer + i;
+      c[i] = s;
+      if (x < E) s += (tot[x] + a.align - 1) / a.align * a.align;
+    }
+    int up = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += y;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane * kPer + i < E) off[lane * kPer + i] = up - s + c[i];
+    if (lane == 31) off[E] = up;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int p = p0 + i * 32 + lane;
+    if (p < a.n_pairs) {
+      int at = -1;
+      if (e[i] >= 0) {
+        at = off[e[i]] + before[e[i]] + wcnt[warp * E + e[i]] + rank[i];
+        a.pair[at] = p;
+      }
+      a.pos[p] = at;
+    }
+  }
+  // rows that no pair takes
+  for (int x = blockIdx.x; x < E; x += gridDim.x)
+    for (int r = off[x] + tot[x] + threadIdx.x; r < off[x + 1]; r += blockDim.x) a.pair[r] = -1;
+  for (int r = off[E] + blockIdx.x * blockDim.x + threadIdx.x; r < a.n_rows; r += gridDim.x * blockDim.x) a.pair[r] = -1;
+  if (blockIdx.x == 0) {
+    for (int x = threadIdx.x; x < E; x += blockDim.x) a.counts[x] = tot[x];
+    for (int x = threadIdx.x; x <= E; x += blockDim.x) a.offsets[x] = off[x];
+  }
+}
+
+// ----------------------------------------------------------------- permute
+// A warp per row.  VEC: 16-byte vectors (rows and strides aligned).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, long long ldx,
+                                                      const int32_t* __restrict__ pair, T* __restrict__ rows, int H,
+                                                      int K, int n_rows) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= n_rows) return;
+  const int p = pair[r];
+  const T* src = x + (p >= 0 ? (long long)(p / K) : 0) * ldx;
+  T* dst = rows + (size_t)r * H;
+  if constexpr (VEC) {
+    const int nv = H * (int)sizeof(T) / 16;
+    const uint4* s = reinterpret_cast<const uint4*>(src);
+    uint4* d = reinterpret_cast<uint4*>(dst);
+#pragma unroll 4
+    for (int i = lane; i < nv; i += 32) d[i] = p >= 0 ? __ldg(s + i) : make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll 4
+    for (int i = lane; i < H; i += 32) {
+      T v;
+      if (p >= 0) v = src[i];
+      else memset(&v, 0, sizeof(T));
+      dst[i] = v;
+    }
+  }
+}
+
+// --------------------------------------------------------------- unpermute
+// A thread takes one vector of a token's columns and sums its K rows, all of
+// whose loads it issues first (8 at a time).  The weight of slot k is
+// probs[t,k] (1 without probs) times scale[ids[t,k]] (with scale).
+template <int TYPE_IN, int TYPE, bool VEC>
+__global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE_IN>::T* __restrict__ rows,
+                                                        const int32_t* __restrict__ pos,
+                                                        const float* __restrict__ probs,
+                                                        const int32_t* __restrict__ ids,
+                                                        const float* __restrict__ scale,
+                                                        typename Elem<TYPE>::T* __restrict__ out, long long ldo,
+                                                        int H, int K, int per_token) {
+  using EI = Elem<TYPE_IN>;
+  using E = Elem<TYPE>;
+  constexpr int V = VEC ? 8 : 1;  // values per thread
+  pdl_wait();
+  pdl_trigger();
+  const long long t = blockIdx.x / per_token;
+  const int c = (blockIdx.x % per_token * 128 + threadIdx.x) * V;
+  if (c >= H) return;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  for (int k0 = 0; k0 < K; k0 += 8) {
+    int at[8];
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      at[j] = k0 + j < K ? __ldg(pos + t * K + k0 + j) : -1;
+      w[j] = k0 + j < K && probs ? __ldg(probs + t * K + k0 + j) : 1.f;
+      if (scale && at[j] >= 0) w[j] *= __ldg(scale + __ldg(ids + t * K + k0 + j));
+    }
+    if constexpr (VEC) {
+      constexpr int N = 8 / EI::kVec;
+      uint4 u[8][N];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (at[j] >= 0) u[j][n] = __ldg(reinterpret_cast<const uint4*>(rows + (size_t)at[j] * H + c) + n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (at[j] < 0) continue;
+        float v[8];
+#pragma unroll
+        for (int n = 0; n < N; ++n) EI::unpack(u[j][n], v + n * EI::kVec);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], v[i], acc[i]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at[j] >= 0) acc[0] = fmaf(w[j], EI::get(rows[(size_t)at[j] * H + c]), acc[0]);
+    }
+  }
+  typename E::T* o = out + t * ldo + c;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int n = 0; n < 8 / E::kVec; ++n) reinterpret_cast<uint4*>(o)[n] = E::pack(acc + n * E::kVec);
+  } else {
+    *o = E::put(acc[0]);
+  }
+}
+
+// ------------------------------------------------------- unpermute gradient
+// A warp per pair: reads the pair's row and the token's gradient once, writes
+// the row's gradient and the weight's.  The K warps of a token share its
+// gradient row through L1.  The warp also clears the row of its own index
+// when no pair takes it (there are at least as many rows as pairs).
+template <int TYPE, bool VEC>
+__global__ void __launch_bounds__(256) unpermute_grad_kernel(const typename Elem<TYPE>::T* __restrict__ dout,
+                                                             long long ldd,
+                                                             const typename Elem<TYPE>::T* __restrict__ rows,
+                                                             const int32_t* __restrict__ pos,
+                                                             const int32_t* __restrict__ pair,
+                                                             const float* __restrict__ probs,
+                                                             typename Elem<TYPE>::T* __restrict__ drows,
+                                                             float* __restrict__ dprobs, int H, int K, int n_pairs,
+                                                             int n_rows) {
+  using E = Elem<TYPE>;
+  using T = typename E::T;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int i0 = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int nv = H / E::kVec;
+  if (i0 < n_pairs) {
+    const int at = pos[i0];
+    const float w = probs ? probs[i0] : 1.f;
+    const T* g = dout + (long long)(i0 / K) * ldd;
+    float dot = 0.f;
+    if (at >= 0) {
+      const T* y = rows + (size_t)at * H;
+      T* d = drows ? drows + (size_t)at * H : nullptr;
+      if constexpr (VEC) {
+#pragma unroll 4
+        for (int i = lane; i < nv; i += 32) {
+          float a[E::kVec], b[E::kVec];
+          E::unpack(__ldg(reinterpret_cast<const uint4*>(g) + i), a);
+          if (dprobs) {
+            E::unpack(__ldg(reinterpret_cast<const uint4*>(y) + i), b);
+#pragma unroll
+            for (int j = 0; j < E::kVec; ++j) dot = fmaf(a[j], b[j], dot);
+          }
+          if (d) {
+#pragma unroll
+            for (int j = 0; j < E::kVec; ++j) a[j] *= w;
+            reinterpret_cast<uint4*>(d)[i] = E::pack(a);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = lane; i < H; i += 32) {
+          const float a = E::get(g[i]);
+          if (dprobs) dot = fmaf(a, E::get(y[i]), dot);
+          if (d) d[i] = E::put(a * w);
+        }
+      }
+    }
+    if (dprobs) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane == 0) dprobs[i0] = dot;
+    }
+  }
+  if (drows && i0 < n_rows && pair[i0] < 0) {
+    T* d = drows + (size_t)i0 * H;
+    if constexpr (VEC) {
+      for (int i = lane; i < nv; i += 32) reinterpret_cast<uint4*>(d)[i] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int i = lane; i < H; i += 32) d[i] = E::put(0.f);
+    }
+  }
+}
+
+bool rows_aligned(const void* p, long long ld, size_t s) { return ((uintptr_t)p & 15) == 0 && (size_t)ld * s % 16 == 0; }
+
+}  // namespace
+
+// Pairs up to which one CTA sorts (ITEMS pairs per thread), and the chunk of
+// the larger sorts, whose two launches read the ids twice.
+constexpr int kSortOne = 4096;
+
+int sort_chunk(long long n_pairs) { return n_pairs <= (1 << 19) ? 1024 : 8192; }
+
+size_t sort_chunk_ints(long long n_pairs, int E) {
+  if (n_pairs <= kSortOne) return 0;
+  const int c = sort_chunk(n_pairs);
+  return (size_t)((n_pairs + c - 1) / c) * E;
+}
+
+cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, int32_t* pos, int32_t* pair, int E,
+                        int n_pairs, int align, int n_rows, int32_t* chunk_cnt, int* err, cudaStream_t s) {
+  SortArgs a{ids, offsets, counts, pos, pair, chunk_cnt, err, n_pairs, E, align, n_rows, 0};
+  const bool one = n_pairs <= kSortOne;
+  const int items = one ? (n_pairs <= 1024 ? 1 : 4) : sort_chunk(n_pairs) / 1024;
+  const int threads = one ? std::min(1024, std::max(256, (n_pairs + 31) / 32 * 32)) : 1024;
+  a.chunk = items * threads;
+  const int grid = std::max(1, (n_pairs + a.chunk - 1) / a.chunk);
+  const size_t smem = (size_t)(threads / 32 * E + 3 * E + 1) * 4;
+  if (!one) {
+    const cudaError_t st = launch_pdl(sort_count_kernel, dim3(grid), dim3(1024), 0, s, a);
+    if (st != cudaSuccess) return st;
+  }
+  switch (items) {
+    case 1: return launch_pdl(sort_place_kernel<1>, dim3(grid), dim3(threads), smem, s, a);
+    case 4: return launch_pdl(sort_place_kernel<4>, dim3(grid), dim3(threads), smem, s, a);
+    default: return launch_pdl(sort_place_kernel<8>, dim3(grid), dim3(threads), smem, s, a);
+  }
+}
+
+cudaError_t launch_permute(int type, const void* x, long long ldx, const int32_t* pair, void* rows, int H, int K,
+                           int n_rows, cudaStream_t s) {
+  const size_t sz = elem_bytes(type);
+  const bool vec = rows_aligned(x, ldx, sz) && rows_aligned(rows, H, sz);
+  const dim3 grid((n_rows + 7) / 8), block(256);
+  if (sz == 4)
+    return vec ? launch_pdl(permute_kernel<uint32_t, true>, grid, block, 0, s, (const uint32_t*)x, ldx, pair, (uint32_t*)rows, H, K, n_rows)
+               : launch_pdl(permute_kernel<uint32_t, false>, grid, block, 0, s, (const uint32_t*)x, ldx, pair, (uint32_t*)rows, H, K, n_rows);
+  return vec ? launch_pdl(permute_kernel<uint16_t, true>, grid, block, 0, s, (const uint16_t*)x, ldx, pair, (uint16_t*)rows, H, K, n_rows)
+             : launch_pdl(permute_kernel<uint16_t, false>, grid, block, 0, s, (const uint16_t*)x, ldx, pair, (uint16_t*)rows, H, K, n_rows);
+}
+
+namespace {
+template <int TI, int TO>
+cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* probs, const int32_t* ids,
+                         const float* scale, void* out, long long ldo, int H, int K, int T, cudaStream_t s) {
+  using I = typename Elem<TI>::T;
+  using O = typename Elem<TO>::T;
+  const bool vec = H % 8 == 0 && rows_aligned(rows, H, sizeof(I)) && rows_aligned(out, ldo, sizeof(O));
+  const int per = (H + 128 * (vec ? 8 : 1) - 1) / (128 * (vec ? 8 : 1));
+  const dim3 grid((unsigned)((long long)T * per)), block(128);
+  return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per)
+             : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per);
+}
+
+template <int TYPE>
+cudaError_t unpermute_grad_as(const void* dout, long long ldd, const void* rows, const int32_t* pos,
+                              const int32_t* pair, const float* probs, void* drows, float* dprobs, int H, int K,
+                              int n_pairs, int n_rows, cudaStream_t s) {
+  using T = typename Elem<TYPE>::T;
+  const bool vec = rows_aligned(dout, ldd, sizeof(T)) && (!rows || rows_aligned(rows, H, sizeof(T))) &&
+                   (!drows || rows_aligned(drows, H, sizeof(T))) && (size_t)H * sizeof(T) % 16 == 0;
+  const dim3 grid((std::max(n_pairs, drows ? n_rows : 0) + 7) / 8), block(256);
+  return vec ? launch_pdl(unpermute_grad_kernel<TYPE, true>, grid, block, 0, s, (const T*)dout, ldd, (const T*)rows, pos, pair, probs, (T*)drows, dprobs, H, K, n_pairs, n_rows)
+             : launch_pdl(unpermute_grad_kernel<TYPE, false>, grid, block, 0, s, (const T*)dout, ldd, (const T*)rows, pos, pair, probs, (T*)drows, dprobs, H, K, n_pairs, n_rows);
+}
+}  // namespace
+
+cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, const float* probs, void* out,
+                             long long ldo, int H, int K, int T, cudaStream_t s) {
+  switch (type) {
+    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
+    case kF16: return unpermute_as<kF16, kF16>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
+    default: return unpermute_as<kBF16, kBF16>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
+  }
+}
+
+cudaError_t launch_unpermute_f32(int type, const float* rows, const int32_t* pos, const float* probs,
+                                 const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                 cudaStream_t s) {
+  switch (type) {
+    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
+    case kF16: return unpermute_as<kF32, kF16>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
+    default: return unpermute_as<kF32, kBF16>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
+  }
+}
+
+cudaError_t launch_unpermute_grad(int type, const void* dout, long long ldd, const void* rows, const int32_t* pos,
+                                  const int32_t* pair, const float* probs, void* drows, float* dprobs, int H, int K,
+                                  int T, int n_rows, cudaStream_t s) {
+  switch (type) {
+    case kF32: return unpermute_grad_as<kF32>(dout, ldd, rows, pos, pair, probs, drows, dprobs, H, K, T * K, n_rows, s);
+    case kF16: return unpermute_grad_as<kF16>(dout, ldd, rows, pos, pair, probs, drows, dprobs, H, K, T * K, n_rows, s);
+    default: return unpermute_grad_as<kBF16>(dout, ldd, rows, pos, pair, probs, drows, dprobs, H, K, T * K, n_rows, s);
+  }
+}
+
+}  // namespace mrml

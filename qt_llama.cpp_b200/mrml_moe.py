@@ -31,10 +31,11 @@ MRML_ERR_INVALID_ARGUMENT = -1
 MRML_Q4_0 = 2
 MRML_Q8_0 = 8
 MRML_PACKED = 0x100
+MRML_F32, MRML_F16, MRML_BF16 = 0, 1, 30
 
 # Every symbol include/mrml_moe.h declares, with its ctypes signature.
 _c = ctypes
-_vp, _i, _sz, _f = _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_float
+_vp, _i, _sz, _f, _i64 = _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_float, _c.c_int64
 SIGNATURES = {
     "mrml_moe_version": (_i, []),
     "mrml_moe_status_string": (_c.c_char_p, [_i]),
@@ -90,6 +91,23 @@ SIGNATURES = {
                                   _c.POINTER(_c.c_uint64), _c.POINTER(_c.c_uint64)]),
     "mrml_moe_gguf_meta_u32": (_i, [_vp, _c.c_char_p, _c.POINTER(_c.c_uint32)]),
     "mrml_moe_gguf_read": (_i, [_vp, _c.c_char_p, _vp, _sz]),
+    "mrml_moe_sorted_rows": (_i, [_i] * 4),
+    "mrml_moe_sort_workspace_bytes": (_sz, [_i] * 3),
+    "mrml_moe_sort": (_i, [_vp] * 5 + [_i] * 4 + [_vp, _sz, _vp]),
+    "mrml_moe_permute": (_i, [_i, _vp, _i64, _vp, _vp, _i, _i, _i, _vp]),
+    "mrml_moe_permute_grad": (_i, [_i, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
+    "mrml_moe_unpermute": (_i, [_i, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
+    "mrml_moe_unpermute_grad": (_i, [_i, _vp, _i64] + [_vp] * 6 + [_i] * 4 + [_vp]),
+    "mrml_moe_mx4_bytes": (_sz, [_i] * 3),
+    "mrml_moe_mx4_quantize": (_i, [_i, _vp, _i64, _i64, _vp, _i, _i, _i, _i, _vp]),
+    "mrml_moe_mx4_quantize_both": (_i, [_i, _vp, _i64, _vp, _vp, _i, _i, _vp]),
+    "mrml_moe_mx4_dequantize": (_i, [_i, _vp, _vp, _i64, _i64, _i, _i, _i, _i, _vp]),
+    "mrml_moe_mx4_matmul_workspace_bytes": (_sz, [_i] * 3),
+    "mrml_moe_mx4_matmul": (_i, [_i, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
+    "mrml_moe_mx4_linear_workspace_bytes": (_sz, [_i] * 3),
+    "mrml_moe_mx4_linear": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
+    "mrml_moe_mx4_experts_workspace_bytes": (_sz, [_i] * 5),
+    "mrml_moe_mx4_experts": (_i, [_i] + [_vp] * 6 + [_i64, _vp, _i64] + [_i] * 5 + [_vp, _sz, _vp]),
 }
 
 
@@ -386,6 +404,214 @@ def quantize(wtype, src, dst, stream=None):
     lib = load_library()
     fn = lib.mrml_moe_quantize_q4_0 if wtype == MRML_Q4_0 else lib.mrml_moe_quantize_q8_0
     _check("mrml_moe_quantize", fn(_ptr(src), _ptr(dst), src.numel(), _stream_ptr(stream)))
+
+
+# ---- Tokens sorted by expert and back (rows: f32, f16 or bf16 tensors with
+# contiguous columns; their row strides are taken from the tensors).
+
+
+def _float_type(t) -> int:
+    import torch
+
+    types = {torch.float32: MRML_F32, torch.float16: MRML_F16, torch.bfloat16: MRML_BF16}
+    assert t.dtype in types, f"unsupported element type {t.dtype}"
+    return types[t.dtype]
+
+
+def _ld(t) -> int:
+    """Row stride in elements of a tensor whose last axis is contiguous."""
+    assert t.stride(-1) == 1 or t.shape[-1] == 1, "columns must be contiguous"
+    return t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]
+
+
+def _check_ints(*tensors):
+    import torch
+
+    assert all(t is None or (t.dtype == torch.int32 and t.is_contiguous()) for t in tensors), "int32, contiguous"
+
+
+def _check_f32(*tensors):
+    import torch
+
+    assert all(t is None or (t.dtype == torch.float32 and t.is_contiguous()) for t in tensors), "f32, contiguous"
+
+
+def _zeroed(nbytes: int, device):
+    import torch
+
+    if nbytes == 0:
+        raise MoeError("workspace size", MRML_ERR_INVALID_ARGUMENT, "invalid argument")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device or "cuda")
+
+
+def sorted_rows(E, K, T, align=1) -> int:
+    """Rows of the sorted order (an upper bound when align > 1)."""
+    n = load_library().mrml_moe_sorted_rows(E, K, T, align)
+    if n < 0:
+        raise MoeError("mrml_moe_sorted_rows", n, "invalid argument")
+    return n
+
+
+def new_sort_workspace(E, K, T, device=None):
+    return _zeroed(load_library().mrml_moe_sort_workspace_bytes(E, K, T), device)
+
+
+def sort(ids, offsets, counts, pos, pair, E, K, T, align, ws, stream=None):
+    """mrml_moe_sort: the (token, slot) pairs in expert order."""
+    _check_ints(ids, offsets, counts, pos, pair)
+    assert ids.numel() == T * K and pos.numel() == T * K
+    assert offsets.numel() == E + 1 and counts.numel() == E
+    assert pair.numel() >= sorted_rows(E, K, T, align)
+    _check("mrml_moe_sort",
+           load_library().mrml_moe_sort(_ptr(ids), _ptr(offsets), _ptr(counts), _ptr(pos), _ptr(pair), E, K, T, align,
+                                        _ptr(ws), ws.numel(), _stream_ptr(stream)))
+
+
+def permute(x, pair, rows, H, K, stream=None):
+    """mrml_moe_permute: rows[r] = x[pair[r] / K] (zero where pair[r] is -1)."""
+    _check_ints(pair)
+    assert x.shape[-1] == H and rows.shape == (pair.numel(), H) and rows.is_contiguous() and rows.dtype == x.dtype
+    _check("mrml_moe_permute",
+           load_library().mrml_moe_permute(_float_type(x), _ptr(x), _ld(x), _ptr(pair), _ptr(rows), H, K,
+                                           pair.numel(), _stream_ptr(stream)))
+
+
+def permute_grad(drows, pos, dx, H, K, T, stream=None):
+    """mrml_moe_permute_grad: dx[t] = sum_k drows[pos[t,k]]."""
+    _check_ints(pos)
+    assert drows.shape[-1] == H and drows.is_contiguous() and pos.numel() == T * K
+    assert dx.shape == (T, H) and dx.dtype == drows.dtype
+    _check("mrml_moe_permute_grad",
+           load_library().mrml_moe_permute_grad(_float_type(dx), _ptr(drows), _ptr(pos), _ptr(dx), _ld(dx), H, K, T,
+                                                _stream_ptr(stream)))
+
+
+def unpermute(rows, pos, probs, out, H, K, T, stream=None):
+    """mrml_moe_unpermute: out[t] = sum_k probs[t,k] rows[pos[t,k]] (probs None: 1)."""
+    _check_ints(pos)
+    _check_f32(probs)
+    assert rows.shape[-1] == H and rows.is_contiguous() and pos.numel() == T * K
+    assert out.shape == (T, H) and out.dtype == rows.dtype and (probs is None or probs.numel() == T * K)
+    _check("mrml_moe_unpermute",
+           load_library().mrml_moe_unpermute(_float_type(out), _ptr(rows), _ptr(pos), _ptr(probs), _ptr(out), _ld(out),
+                                             H, K, T, _stream_ptr(stream)))
+
+
+def unpermute_grad(dout, rows, pos, pair, probs, drows, dprobs, H, K, T, stream=None):
+    """mrml_moe_unpermute_grad: the gradients of the rows and of the weights
+    (either may be None)."""
+    _check_ints(pos, pair)
+    _check_f32(probs, dprobs)
+    assert dout.shape == (T, H) and pos.numel() == T * K
+    assert all(t is None or t.numel() == T * K for t in (probs, dprobs))
+    assert all(t is None or (t.shape[-1] == H and t.is_contiguous() and t.dtype == dout.dtype) for t in (rows, drows))
+    assert drows is None or drows.shape[0] == pair.numel()
+    _check("mrml_moe_unpermute_grad",
+           load_library().mrml_moe_unpermute_grad(_float_type(dout), _ptr(dout), _ld(dout), _ptr(rows), _ptr(pos),
+                                                  _ptr(pair), _ptr(probs), _ptr(drows), _ptr(dprobs), H, K, T,
+                                                  0 if drows is None else drows.shape[0], _stream_ptr(stream)))
+
+
+# ---- MXFP4 matrices: uint8 buffers in the library's own layout.
+
+
+def mx4_bytes(rows, cols, matrices=1) -> int:
+    return int(load_library().mrml_moe_mx4_bytes(rows, cols, matrices))
+
+
+def new_mx4(rows, cols, matrices=1, device=None):
+    """An uninitialised buffer for `matrices` quantised matrices of rows x cols."""
+    import torch
+
+    return torch.empty(mx4_bytes(rows, cols, matrices), dtype=torch.uint8, device=device or "cuda")
+
+
+def _check_mx4(q, rows, cols, matrices=1):
+    import torch
+
+    assert q.dtype == torch.uint8 and q.is_contiguous() and q.numel() >= mx4_bytes(rows, cols, matrices)
+
+
+def mx4_quantize(src, dst, rows, cols, matrices=1, gated=False, wtype=None, stream=None):
+    """mrml_moe_mx4_quantize: src [matrices][rows][cols] (f32, f16 or bf16; with
+    wtype, a uint8 tensor of GGUF blocks) into dst."""
+    _check_mx4(dst, rows, cols, matrices)
+    if wtype is None:
+        assert tuple(src.shape) in ((rows, cols), (matrices, rows, cols)) and (src.dim() == 3 or matrices == 1)
+        args = (_float_type(src), _ptr(src), _ld(src), src.stride(0) if src.dim() == 3 else 0)
+    else:
+        bb = 18 if wtype == MRML_Q4_0 else 34
+        assert src.is_contiguous() and src.numel() == matrices * rows * (cols // 32) * bb
+        args = (wtype, _ptr(src), cols, rows * cols)
+    _check("mrml_moe_mx4_quantize",
+           load_library().mrml_moe_mx4_quantize(*args, _ptr(dst), rows, cols, matrices, int(gated),
+                                                _stream_ptr(stream)))
+
+
+def mx4_quantize_both(src, dst, dst_t, rows, cols, stream=None):
+    """mrml_moe_mx4_quantize_both: src [rows][cols] and its transpose, each
+    quantised along its own rows, in one read."""
+    assert tuple(src.shape) == (rows, cols)
+    _check_mx4(dst, rows, cols)
+    _check_mx4(dst_t, cols, rows)
+    _check("mrml_moe_mx4_quantize_both",
+           load_library().mrml_moe_mx4_quantize_both(_float_type(src), _ptr(src), _ld(src), _ptr(dst), _ptr(dst_t),
+                                                     rows, cols, _stream_ptr(stream)))
+
+
+def mx4_dequantize(src, dst, rows, cols, matrices=1, gated=False, stream=None):
+    """mrml_moe_mx4_dequantize: the values src stands for."""
+    _check_mx4(src, rows, cols, matrices)
+    assert tuple(dst.shape) in ((rows, cols), (matrices, rows, cols)) and (dst.dim() == 3 or matrices == 1)
+    _check("mrml_moe_mx4_dequantize",
+           load_library().mrml_moe_mx4_dequantize(_float_type(dst), _ptr(src), _ptr(dst), _ld(dst),
+                                                  dst.stride(0) if dst.dim() == 3 else 0, rows, cols, matrices,
+                                                  int(gated), _stream_ptr(stream)))
+
+
+def new_mx4_matmul_workspace(M, N, K, device=None):
+    return _zeroed(load_library().mrml_moe_mx4_matmul_workspace_bytes(M, N, K), device)
+
+
+def mx4_matmul(a, b, out, M, N, K, ws, stream=None):
+    """mrml_moe_mx4_matmul: out [M][N] = a [M][K] b [N][K]^T of quantised matrices."""
+    _check_mx4(a, M, K)
+    _check_mx4(b, N, K)
+    assert tuple(out.shape) == (M, N)
+    _check("mrml_moe_mx4_matmul",
+           load_library().mrml_moe_mx4_matmul(_float_type(out), _ptr(a), _ptr(b), _ptr(out), _ld(out), M, N, K,
+                                              _ptr(ws), ws.numel(), _stream_ptr(stream)))
+
+
+def new_mx4_linear_workspace(T, N, K, device=None):
+    return _zeroed(load_library().mrml_moe_mx4_linear_workspace_bytes(T, N, K), device)
+
+
+def mx4_linear(x, w, out, T, N, K, ws, stream=None):
+    """mrml_moe_mx4_linear: out [T][N] = Q(x) [T][K] w [N][K]^T."""
+    _check_mx4(w, N, K)
+    assert tuple(x.shape) == (T, K) and tuple(out.shape) == (T, N) and x.dtype == out.dtype
+    _check("mrml_moe_mx4_linear",
+           load_library().mrml_moe_mx4_linear(_float_type(x), _ptr(x), _ld(x), _ptr(w), _ptr(out), _ld(out), T, N, K,
+                                              _ptr(ws), ws.numel(), _stream_ptr(stream)))
+
+
+def new_mx4_experts_workspace(H, I, E, K, T, device=None):
+    return _zeroed(load_library().mrml_moe_mx4_experts_workspace_bytes(H, I, E, K, T), device)
+
+
+def mx4_experts(gate_up, down, ids, probs, down_scale, x, out, H, I, E, K, T, ws, stream=None):
+    """mrml_moe_mx4_experts: the experts and the combine on MXFP4 weights."""
+    _check_mx4(gate_up, 2 * I, H, E)
+    _check_mx4(down, H, I, E)
+    _check_ints(ids)
+    _check_f32(probs, down_scale)
+    assert ids.numel() == T * K and probs.numel() == T * K and (down_scale is None or down_scale.numel() == E)
+    assert tuple(x.shape) == (T, H) and tuple(out.shape) == (T, H) and x.dtype == out.dtype
+    _check("mrml_moe_mx4_experts",
+           load_library().mrml_moe_mx4_experts(_float_type(x), _ptr(gate_up), _ptr(down), _ptr(ids), _ptr(probs),
+                                               _ptr(down_scale), _ptr(x), _ld(x), _ptr(out), _ld(out), H, I, E, K, T,
+                                               _ptr(ws), ws.numel(), _stream_ptr(stream)))
 
 
 OPTION_EXPERT_PATH = 1
