@@ -206,10 +206,11 @@ cudaError_t launch_permute(int type, const void* x, long long ldx, const int32_t
                            int n_rows, cudaStream_t s);
 cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, const float* probs, void* out,
                              long long ldo, int H, int K, int T, cudaStream_t s);
-// The same from f32 rows, with the weights times scale[ids] (scale may be null).
-cudaError_t launch_unpermute_f32(int type, const float* rows, const int32_t* pos, const float* probs,
-                                 const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
-                                 cudaStream_t s);
+// The same from the expert layer's down products (f32 rows), with the weights
+// times scale[ids] (scale may be null).
+cudaError_t launch_combine_rows(int type, const float* rows, const int32_t* pos, const float* probs,
+                                const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                cudaStream_t s);
 cudaError_t launch_unpermute_grad(int type, const void* dout, long long ldd, const void* rows, const int32_t* pos,
                                   const int32_t* pair, const float* probs, void* drows, float* dprobs, int H, int K,
                                   int T, int n_rows, cudaStream_t s);

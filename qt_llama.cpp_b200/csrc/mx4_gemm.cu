@@ -18,7 +18,7 @@
 //              format is the shared-memory operand layout, mx4.cuh)
 //   warp 1     TMEM allocation; lane 0 copies the chunk's scales to tensor
 //              memory and issues the MMAs
-//   warps 4-7  epilogue, on the other of two accumulators
+//   warps 4-11 epilogue, on the other of two accumulators
 // Scales live in tensor memory per shared-memory stage, so a stage's scales
 // are overwritten only after the MMAs that read them have completed.
 // Every wait is bounded; on a timeout the CTA records the error, drains its
@@ -40,9 +40,9 @@ using tc::wait_bar;
 
 constexpr int kStages = 5;
 constexpr int kStageBytes = 2 * kMxChunkBytes;
-constexpr int kThreads = 256;
-constexpr int kExPitch = 65;                        // f32 per row of the GeGLU exchange
-constexpr int kExBytes = kMxRows * kExPitch * 4;    // 128 rows x 64 tokens
+constexpr int kThreads = 384;
+constexpr int kExPitch = 33;                          // f32 per row of the GeGLU exchange
+constexpr int kExBytes = 2 * kMxRows * kExPitch * 4;  // two groups' 128 rows x 32 tokens
 constexpr uint32_t kAcc0 = 0, kAccCols = 128;       // two accumulators of 128 columns
 constexpr uint32_t kSf0 = 256, kSfCols = 16;        // scales: 8 + 8 columns per stage
 
@@ -107,15 +107,28 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
-// Whether `ok` holds in all 128 threads of the epilogue (a barrier of theirs).
-__device__ __forceinline__ bool all_epilogue(bool ok) {
+// Barrier of the 128 threads of an epilogue group, and whether `ok` holds in
+// all of them.
+__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool all_of_group(bool ok, int id) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)ok)
+      : "r"((uint32_t)ok), "r"(id)
       : "memory");
   return r != 0;
+}
+
+// One lane of a converged warp.  The compiler knows such a branch to have a
+// single thread and keeps the operands of the tensor-core instructions in
+// uniform registers; under `lane == 0` it serialises every one of them over
+// the warp, about 90 cycles each (a K chunk of 128 tokens took 1500 cycles
+// instead of 800).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // A unit: its expert, weight tile, first token row and tokens.
@@ -161,6 +174,22 @@ __device__ __forceinline__ float geglu(float g, float u) {
   return __fdividef(g, 1.f + __expf(-z2)) * u;
 }
 
+// A chunk of n blocks (even): its scales to tensor memory, then n / 2 MMAs.
+template <int n>
+__device__ __forceinline__ void chunk_mma(uint32_t acc, uint32_t wa, uint32_t xa, uint32_t sf, uint32_t id0,
+                                          uint32_t id2, bool add) {
+  constexpr int kGroups = (n + 3) / 4;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    copy_scales(sf + 4 * g, wa + 512 * g);
+    copy_scales(sf + 8 + 4 * g, xa + 512 * g);
+  }
+  const uint64_t da = desc(wa + 512 * kGroups, n * 128), db = desc(xa + 512 * kGroups, n * 128);
+#pragma unroll
+  for (int j = 0; j < n / 2; ++j)
+    mma_mxf4(acc, da + j * 16, db + j * 16, j & 1 ? id2 : id0, sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, add || j > 0);
+}
+
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
 
 template <int MODE>
@@ -178,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B->acc_full[i], 1);
-      mbar_init(&B->acc_empty[i], 4);
+      mbar_init(&B->acc_empty[i], 8);
     }
     mbar_init(&B->drain, 1);
     B->abort = 0;
@@ -219,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   const size_t tile_bytes = mx_tile_bytes(P.nb);
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -254,29 +283,32 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       int s = 0, a = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
       for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
         const Unit U = unit_of(P, B, u);
         const int N = (U.n + 15) & ~15;
+        const uint32_t id0 = idesc(N, 0), id2 = idesc(N, 2);
         if (!(ok = wait_bar(&B->acc_empty[a], aph ^ 1, B, P.err))) break;
         fence_after();
         const uint32_t acc = tmem + kAcc0 + a * kAccCols;
         for (int c = 0; c < nc; ++c) {
           if (!(ok = wait_bar(&B->full[s], ph, B, P.err))) break;
           fence_after();
-          const int n = min(kMxChunk, P.nb - c * kMxChunk);
           const uint32_t wa = smem_u32(ring + s * kStageBytes), xa = wa + kMxChunkBytes;
-          const uint32_t sf = tmem + kSf0 + s * kSfCols, sb = mx_scale_bytes(n);
-          for (uint32_t g = 0; g < sb; g += 512) {
-            copy_scales(sf + g / 128, wa + g);
-            copy_scales(sf + 8 + g / 128, xa + g);
+          const uint32_t sf = tmem + kSf0 + s * kSfCols;
+          const int n = P.nb - c * kMxChunk;
+          if (n >= kMxChunk) {
+            chunk_mma<kMxChunk>(acc, wa, xa, sf, id0, id2, c > 0);
+          } else if (n == 2) {
+            chunk_mma<2>(acc, wa, xa, sf, id0, id2, c > 0);
+          } else if (n == 4) {
+            chunk_mma<4>(acc, wa, xa, sf, id0, id2, c > 0);
+          } else {
+            chunk_mma<6>(acc, wa, xa, sf, id0, id2, c > 0);
           }
-          for (int j = 0; j < n / 2; ++j)
-            mma_mxf4(acc, desc(wa + sb + j * 256, n * 128), desc(xa + sb + j * 256, n * 128), idesc(N, (j & 1) * 2),
-                     sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, c + j > 0);
           mma_commit(&B->empty[s]);
           if (++s == kStages) {
             s = 0;
@@ -291,60 +323,74 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       mbar_wait_bounded(&B->drain, 0, nullptr);
     }
   } else if (warp >= 4) {
-    const int q = warp & 3;
+    // Two groups of four warps; a group's warp q reads the lanes 32q..32q+31
+    // of tensor memory (weight rows), the groups take 32 columns (tokens) in
+    // turn.
+    const int q = warp & 3, grp = (warp - 4) >> 2;
     int a = 0;
     uint32_t aph = 0;
     for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
       const Unit U = unit_of(P, B, u);
       bool ok = wait_bar(&B->acc_full[a], aph, B, P.err);
-      // All lanes leave together; all four warps where they meet at barriers.
-      if constexpr (MODE == kModeGated) ok = all_epilogue(ok);
+      // All lanes leave together; the four warps of a group where they meet
+      // at barriers.
+      if constexpr (MODE == kModeGated) ok = all_of_group(ok, 1 + grp);
       else ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
       const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + kAcc0 + a * kAccCols;
       uint32_t r[32];
       if constexpr (MODE == kModeGated) {
-        // 64 tokens at a time: all rows to shared memory (rows 0..63 gate,
-        // 64..127 up), then a thread per (token, block of 32 outputs).
-        const int tid = threadIdx.x - 128;
+        // 32 tokens at a time: all rows to shared memory (rows 0..63 gate,
+        // 64..127 up), then two threads per (token, block of 32 outputs).
         const int nba = mx_blocks(P.n_out);
-        for (int c0 = 0; c0 < U.n; c0 += 64) {
-#pragma unroll
-          for (int h = 0; h < 64; h += 32) {
-            if (c0 + h >= U.n) break;
-            tmem_ld32(acc + c0 + h, r);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ex[(32 * q + lane) * kExPitch + h + i] = __uint_as_float(r[i]);
-          }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          const int t = tid & 63, b = tid >> 6;
-          const int row = U.row0 + c0 + t, blk = U.wt * 2 + b;
-          if (c0 + t < U.n && blk < nba) {
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              v[i] = geglu(ex[(32 * b + i) * kExPitch + t], ex[(64 + 32 * b + i) * kExPitch + t]);
-            uint4 codes;
-            const uint32_t s = mx_quantize32(v, codes);
-            uint8_t* tile = P.act + (size_t)(row / kMxRows) * mx_tile_bytes(nba);
-            *reinterpret_cast<uint4*>(tile + mx_code_offset(nba, row % kMxRows, blk)) = codes;
-            tile[mx_scale_offset(row % kMxRows, blk)] = (uint8_t)s;
-          }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-        }
-      } else {
-        using E = Elem<MODE == kModeF32 ? kF32 : MODE == kModeF16 ? kF16 : kBF16>;
-        const int f = U.wt * kMxRows + 32 * q + lane;
-        typename E::T* out = static_cast<typename E::T*>(P.out) + (long long)U.row0 * P.ldo + f;
-        for (int c0 = 0; c0 < U.n; c0 += 32) {
+        float* x = ex + grp * (kMxRows * kExPitch);
+        const int half = lane & 1, t = (q & 1) * 16 + (lane >> 1), b = q >> 1, blk = U.wt * 2 + b;
+        const float* xg = x + (32 * b + 16 * half) * kExPitch + t;
+        uint8_t* tile = P.act + (size_t)(U.row0 / kMxRows) * mx_tile_bytes(nba);
+        for (int c0 = 32 * grp; c0 < U.n; c0 += 64) {
           tmem_ld32(acc + c0, r);
           tmem_wait_ld();
-          if (f < P.n_out) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i < U.n) out[(long long)(c0 + i) * P.ldo] = E::put(__uint_as_float(r[i]));
+          for (int i = 0; i < 32; ++i) x[(32 * q + lane) * kExPitch + i] = __uint_as_float(r[i]);
+          group_barrier(1 + grp);
+          float v[16];
+          uint32_t amax = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = geglu(xg[i * kExPitch], xg[(64 + i) * kExPitch]);
+            amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+          }
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          float inv;
+          const uint32_t s = mx_scale(amax, inv);
+          if (c0 + t < U.n && blk < nba) {
+            *reinterpret_cast<uint2*>(tile + mx_code_offset(nba, c0 + t, blk) + 8 * half) =
+                make_uint2(mx_pack8(v, inv), mx_pack8(v + 8, inv));
+            if (half == 0) tile[mx_scale_offset(c0 + t, blk)] = (uint8_t)s;
+          }
+          group_barrier(1 + grp);
+        }
+      } else {
+        const int f = U.wt * kMxRows + 32 * q + lane;
+        for (int c0 = 32 * grp; c0 < U.n; c0 += 64) {
+          tmem_ld32(acc + c0, r);
+          tmem_wait_ld();
+          using E = Elem<MODE == kModeF32 ? kF32 : MODE == kModeF16 ? kF16 : kBF16>;
+          typename E::T* o = static_cast<typename E::T*>(P.out) + (long long)(U.row0 + c0) * P.ldo + f;
+          const int n = f < P.n_out ? min(32, U.n - c0) : 0;
+          if (n == 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              *o = E::put(__uint_as_float(r[i]));
+              o += P.ldo;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (i < n) *o = E::put(__uint_as_float(r[i]));
+              o += P.ldo;
+            }
           }
         }
       }

@@ -301,9 +301,9 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
   MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.x, T, H, K, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, gate_up, w.x, w.offsets, w.counts, E, 0, 2 * I, H, true, nullptr, 0,
                                     w.act, tiles, w.sort.status, s));
-  MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H, nullptr,
-                                    tiles, w.sort.status, s));
-  MRML_LAUNCH(mrml::launch_unpermute_f32(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
+  MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H,
+                                    nullptr, tiles, w.sort.status, s));
+  MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
   return MRML_OK;
 }
 

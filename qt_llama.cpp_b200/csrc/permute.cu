@@ -388,9 +388,9 @@ cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, con
   }
 }
 
-cudaError_t launch_unpermute_f32(int type, const float* rows, const int32_t* pos, const float* probs,
-                                 const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
-                                 cudaStream_t s) {
+cudaError_t launch_combine_rows(int type, const float* rows, const int32_t* pos, const float* probs,
+                                const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                cudaStream_t s) {
   switch (type) {
     case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
     case kF16: return unpermute_as<kF32, kF16>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
