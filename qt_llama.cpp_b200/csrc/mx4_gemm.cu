@@ -64,14 +64,18 @@ struct __align__(8) Bars {
   uint32_t tmem_base;
   int abort;
   int first[kMaxExperts + 1];  // token tiles of earlier experts
+  int row0[kMaxExperts], count[kMaxExperts];  // each expert's first row and rows
 };
-static_assert(sizeof(Bars) <= 2048, "the barrier block must fit its part of shared memory");
-constexpr int kBarBytes = 2048;
+constexpr int kBarBytes = 4096;
+static_assert(sizeof(Bars) <= kBarBytes, "the barrier block must fit its part of shared memory");
 
 // Shared-memory operand descriptor, K-major without swizzle: core matrices of
-// 8 rows x 16 bytes, 128 bytes apart along K and `sbo` along the rows.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46;
+// 8 rows x 16 bytes, 128 bytes apart along K and `sbo` along the rows.  The
+// low word holds the address (in 16-byte units: adding to it moves the
+// operand) and the K distance, the high word the row distance.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return (addr >> 4) | (128 >> 4) << 16; }
+__device__ __forceinline__ uint64_t desc(uint32_t lo, uint32_t sbo) {
+  return (uint64_t)((sbo >> 4) | 1u << 14) << 32 | lo;
 }
 
 // Instruction descriptor of kind::mxf4: E2M1 operands (1), both K-major, E8M0
@@ -92,8 +96,8 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
 
 // 32 lanes x 16 bytes of shared memory to four TMEM columns, the same in each
 // of the four lane quarters.
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t addr) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(addr, 128)) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t lo) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(lo, 128)) : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -120,6 +124,38 @@ __device__ __forceinline__ bool all_of_group(bool ok, int id) {
   return r != 0;
 }
 
+// mbarrier operations and bulk copies on shared-memory addresses.
+__device__ __forceinline__ bool try_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, Bars* B, int* err) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (try_at(bar, parity)) return true;
+    if ((i & 255) == 255 && tc::aborted(B)) return false;
+    if (i > 128) __nanosleep(64);
+  }
+  set_error(err, kDevTimeout);
+  *(volatile int*)&B->abort = 1;
+  return false;
+}
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, Bars* B, int* err) {
+  return try_at(bar, parity) || wait_slow(bar, parity, B, err);
+}
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_at(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // One lane of a converged warp.  The compiler knows such a branch to have a
 // single thread and keeps the operands of the tensor-core instructions in
 // uniform registers; under `lane == 0` it serialises every one of them over
@@ -131,40 +167,43 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// A unit: its expert, weight tile, first token row and tokens.
-struct Unit {
+// The units of a CTA in turn (each role walks them by itself): weight tile,
+// first token row, tokens.  Within an expert, units that follow one another
+// share the weight tile.  The expert only moves forward, by steps through
+// shared memory; searching for it in the offsets in global memory cost each
+// role 1000 to 1700 cycles per unit.
+struct Units {
+  int u, e, first, next;  // unit; expert, its first unit and the next expert's
   int wt, row0, n;
   size_t w_tile;
-};
 
-__device__ __forceinline__ Unit unit_of(const Params& P, const Bars* B, int u) {
-  Unit U;
-  int e = 0, t;
-  if (P.offsets) {
-    // expert: the last with first[e] * w_tiles <= u
-    const int tile = u / P.w_tiles;  // token tile index over all experts, up to the order inside an expert
-    int lo = 0, hi = P.E;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (B->first[mid] <= tile) lo = mid;
-      else hi = mid;
-    }
-    e = lo;
-    const int tt = B->first[e + 1] - B->first[e], r = u - B->first[e] * P.w_tiles;
-    U.wt = r / tt;
-    t = r % tt;
-    U.row0 = P.offsets[e] + t * kMxRows;
-    U.n = min(kMxRows, P.counts[e] - t * kMxRows);
-  } else {
-    const int tt = (P.n_tokens + kMxRows - 1) / kMxRows;
-    U.wt = u / tt;
-    t = u % tt;
-    U.row0 = t * kMxRows;
-    U.n = min(kMxRows, P.n_tokens - U.row0);
+  __device__ __forceinline__ void start(const Params& P, const Bars* B) {
+    u = (int)blockIdx.x;
+    e = 0;
+    first = 0;
+    next = P.offsets ? B->first[1] * P.w_tiles : 0x7fffffff;
   }
-  U.w_tile = (size_t)e * P.w_tiles + U.wt;
-  return U;
-}
+  __device__ __forceinline__ void locate(const Params& P, const Bars* B) {
+    if (P.offsets) {
+      while (u >= next) {  // u is below the last expert's end
+        ++e;
+        first = next;
+        next = B->first[e + 1] * P.w_tiles;
+      }
+      const unsigned tt = (unsigned)(B->first[e + 1] - B->first[e]), r = (unsigned)(u - first);
+      wt = (int)(r / tt);
+      const int t = (int)(r - wt * tt);
+      row0 = B->row0[e] + t * kMxRows;
+      n = min(kMxRows, B->count[e] - t * kMxRows);
+    } else {
+      const unsigned tt = (unsigned)(P.n_tokens + kMxRows - 1) / kMxRows;
+      wt = (int)((unsigned)u / tt);
+      row0 = (int)(u - wt * tt) * kMxRows;
+      n = min(kMxRows, P.n_tokens - row0);
+    }
+    w_tile = (size_t)e * P.w_tiles + wt;
+  }
+};
 
 // gelu_tanh(g) * u; 0.5 g (1 + tanh(z)) = g / (1 + exp(-2z)), which keeps its
 // relative precision for large negative g.  The exponent saturates harmlessly:
@@ -175,19 +214,20 @@ __device__ __forceinline__ float geglu(float g, float u) {
 }
 
 // A chunk of n blocks (even): its scales to tensor memory, then n / 2 MMAs.
+// wa, xa: descriptor low words of the weights' and the tokens' chunk.
 template <int n>
 __device__ __forceinline__ void chunk_mma(uint32_t acc, uint32_t wa, uint32_t xa, uint32_t sf, uint32_t id0,
                                           uint32_t id2, bool add) {
   constexpr int kGroups = (n + 3) / 4;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    copy_scales(sf + 4 * g, wa + 512 * g);
-    copy_scales(sf + 8 + 4 * g, xa + 512 * g);
+    copy_scales(sf + 4 * g, wa + 32 * g);
+    copy_scales(sf + 8 + 4 * g, xa + 32 * g);
   }
-  const uint64_t da = desc(wa + 512 * kGroups, n * 128), db = desc(xa + 512 * kGroups, n * 128);
 #pragma unroll
   for (int j = 0; j < n / 2; ++j)
-    mma_mxf4(acc, da + j * 16, db + j * 16, j & 1 ? id2 : id0, sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, add || j > 0);
+    mma_mxf4(acc, desc(wa + 32 * kGroups + j * 16, n * 128), desc(xa + 32 * kGroups + j * 16, n * 128),
+             j & 1 ? id2 : id0, sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, add || j > 0);
 }
 
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
@@ -226,7 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     for (int i = 0; i < kPer; ++i) {
       const int x = lane * kPer + i;
       c[i] = s;
-      if (x < P.E) s += (P.counts[x] + kMxRows - 1) / kMxRows;
+      if (x < P.E) {
+        const int n = P.counts[x];
+        B->count[x] = n;
+        B->row0[x] = P.offsets[x];
+        s += (n + kMxRows - 1) / kMxRows;
+      }
     }
     int up = s;
 #pragma unroll
@@ -244,33 +289,43 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   fence_after();
   const uint32_t tmem = B->tmem_base;
   const int n_units = (P.offsets ? B->first[P.E] : (P.n_tokens + kMxRows - 1) / kMxRows) * P.w_tiles;
-  const int nc = (P.nb + kMxChunk - 1) / kMxChunk;
   const size_t tile_bytes = mx_tile_bytes(P.nb);
 
+  // The producer's and the issuer's loops run in one thread each, where every
+  // instruction costs its latency: addresses advance instead of being
+  // computed, and whole chunks have constant sizes.
+  const int n_full = P.nb / kMxChunk, n_tail = P.nb % kMxChunk;
+  const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(&B->full[0]), empty0 = smem_u32(&B->empty[0]);
   if (warp == 0) {
     if (elect_one()) {
       int s = 0, issued = 0;
       uint32_t ph = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
-        const Unit U = unit_of(P, B, u);
-        const uint8_t* wsrc = P.w + U.w_tile * tile_bytes;
-        const uint8_t* xsrc = P.x + (size_t)(U.row0 / kMxRows) * tile_bytes;
-        const int groups = ((U.n + 15) & ~15) >> 3;
-        for (int c = 0; c < nc; ++c) {
-          if (!(ok = wait_bar(&B->empty[s], ph ^ 1, B, P.err))) break;
-          const int n = min(kMxChunk, P.nb - c * kMxChunk);
-          const uint32_t wb = mx_chunk_bytes(n), xb = mx_scale_bytes(n) + groups * n * 128;
-          uint8_t* dst = ring + s * kStageBytes;
-          mbar_arrive_expect_tx(&B->full[s], wb + xb);
-          bulk_g2s(dst, wsrc + (size_t)c * kMxChunkBytes, wb, &B->full[s]);
-          bulk_g2s(dst + kMxChunkBytes, xsrc + (size_t)c * kMxChunkBytes, xb, &B->full[s]);
-          ++issued;
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1;
-          }
+      auto load = [&](const uint8_t* w, const uint8_t* x, uint32_t wb, uint32_t xb) {
+        if (!wait_at(empty0 + 8 * s, ph ^ 1, B, P.err)) return false;
+        const uint32_t bar = full0 + 8 * s, dst = ring0 + s * kStageBytes;
+        expect_at(bar, wb + xb);
+        copy_at(dst, w, wb, bar);
+        copy_at(dst + kMxChunkBytes, x, xb, bar);
+        ++issued;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
         }
+        return true;
+      };
+      bool ok = true;
+      Units U;
+      for (U.start(P, B); U.u < n_units && ok; U.u += gridDim.x) {
+        U.locate(P, B);
+        const uint8_t* w = P.w + U.w_tile * tile_bytes;
+        const uint8_t* x = P.x + (size_t)(U.row0 / kMxRows) * tile_bytes;
+        const uint32_t groups = ((U.n + 15) & ~15) >> 3, xb = 1024 + groups * (kMxChunk * 128);
+        for (int c = 0; c < n_full && ok; ++c) {
+          ok = load(w, x, kMxChunkBytes, xb);
+          w += kMxChunkBytes;
+          x += kMxChunkBytes;
+        }
+        if (n_tail && ok) ok = load(w, x, mx_chunk_bytes(n_tail), mx_scale_bytes(n_tail) + groups * (n_tail * 128));
       }
       // Whatever happened, every copy lands before the block gives up its
       // shared memory.
@@ -287,34 +342,30 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       int s = 0, a = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
-        const Unit U = unit_of(P, B, u);
+      Units U;
+      for (U.start(P, B); U.u < n_units && ok; U.u += gridDim.x) {
+        U.locate(P, B);
         const int N = (U.n + 15) & ~15;
         const uint32_t id0 = idesc(N, 0), id2 = idesc(N, 2);
         if (!(ok = wait_bar(&B->acc_empty[a], aph ^ 1, B, P.err))) break;
         fence_after();
         const uint32_t acc = tmem + kAcc0 + a * kAccCols;
-        for (int c = 0; c < nc; ++c) {
-          if (!(ok = wait_bar(&B->full[s], ph, B, P.err))) break;
+        auto chunk = [&](auto issue, bool add) {
+          if (!wait_at(full0 + 8 * s, ph, B, P.err)) return false;
           fence_after();
-          const uint32_t wa = smem_u32(ring + s * kStageBytes), xa = wa + kMxChunkBytes;
-          const uint32_t sf = tmem + kSf0 + s * kSfCols;
-          const int n = P.nb - c * kMxChunk;
-          if (n >= kMxChunk) {
-            chunk_mma<kMxChunk>(acc, wa, xa, sf, id0, id2, c > 0);
-          } else if (n == 2) {
-            chunk_mma<2>(acc, wa, xa, sf, id0, id2, c > 0);
-          } else if (n == 4) {
-            chunk_mma<4>(acc, wa, xa, sf, id0, id2, c > 0);
-          } else {
-            chunk_mma<6>(acc, wa, xa, sf, id0, id2, c > 0);
-          }
+          const uint32_t wa = desc_lo(ring0 + s * kStageBytes);
+          issue(acc, wa, wa + (kMxChunkBytes >> 4), tmem + kSf0 + s * kSfCols, id0, id2, add);
           mma_commit(&B->empty[s]);
           if (++s == kStages) {
             s = 0;
             ph ^= 1;
           }
-        }
+          return true;
+        };
+        for (int c = 0; c < n_full && ok; ++c) ok = chunk(chunk_mma<kMxChunk>, c > 0);
+        if (ok && n_tail == 2) ok = chunk(chunk_mma<2>, n_full > 0);
+        if (ok && n_tail == 4) ok = chunk(chunk_mma<4>, n_full > 0);
+        if (ok && n_tail == 6) ok = chunk(chunk_mma<6>, n_full > 0);
         if (!ok) break;
         mma_commit(&B->acc_full[a]);
         if (a ^= 1; a == 0) aph ^= 1;
@@ -329,8 +380,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     const int q = warp & 3, grp = (warp - 4) >> 2;
     int a = 0;
     uint32_t aph = 0;
-    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
-      const Unit U = unit_of(P, B, u);
+    Units U;
+    for (U.start(P, B); U.u < n_units; U.u += gridDim.x) {
+      U.locate(P, B);
       bool ok = wait_bar(&B->acc_full[a], aph, B, P.err);
       // All lanes leave together; the four warps of a group where they meet
       // at barriers.
