@@ -222,8 +222,12 @@ cudaError_t launch_mx4_quantize_both(int type, const void* x, long long ldx, uin
                                      int cols, cudaStream_t s);
 cudaError_t launch_mx4_dequantize(int type, const uint8_t* src, void* out, long long ldo, long long mstride, int rows,
                                   int cols, int matrices, bool gated, cudaStream_t s);
-cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int32_t* pos, uint8_t* dst, int T, int H,
-                              int K, cudaStream_t s);
+// Tokens quantised into their sorted rows (pos / pair of launch_sort; end: the
+// rows in use, on the device); flat is scratch of mx4_flat_bytes.
+size_t mx4_flat_bytes(int H, int K, int T);
+cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int32_t* pos, const int32_t* pair,
+                              const int32_t* end, uint8_t* dst, uint8_t* flat, int T, int H, int K, int n_rows,
+                              cudaStream_t s);
 // Token rows x (times) weight rows w.  With offsets / counts: E weight
 // matrices, each for its expert's token rows (which start at multiples of
 // 128); without: one matrix and n_tokens rows.  gated: the weights are in the

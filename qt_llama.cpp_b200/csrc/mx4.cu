@@ -12,25 +12,39 @@ namespace {
 
 // The 32 values of block b of a row that starts at `row`; zero past `cols`.
 template <int TYPE>
-__device__ __forceinline__ void load_block(const typename Elem<TYPE>::T* row, int b, int cols, bool vec, float (&v)[32]) {
-  using E = Elem<TYPE>;
+__device__ __forceinline__ void load_block(const typename Elem<TYPE>::T* row, int b, int cols, bool vec,
+                                           MxPart<TYPE, 32>& v) {
   const int c0 = b * 32;
   if (vec && c0 + 32 <= cols) {
     const uint4* p = reinterpret_cast<const uint4*>(row + c0);
-    uint4 u[32 / E::kVec];
 #pragma unroll
-    for (int i = 0; i < 32 / E::kVec; ++i) u[i] = __ldg(p + i);
-#pragma unroll
-    for (int i = 0; i < 32 / E::kVec; ++i) E::unpack(u[i], v + i * E::kVec);
+    for (int i = 0; i < MxPart<TYPE, 32>::kWords / 4; ++i) {
+      const uint4 u = __ldg(p + i);
+      v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+    }
   } else {
+    typename Elem<TYPE>::T t[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? E::get(row[c0 + i]) : 0.f;
+    for (int i = 0; i < 32; ++i) t[i] = c0 + i < cols ? row[c0 + i] : Elem<TYPE>::put(0.f);
+    memcpy(v.w, t, sizeof(v.w));
   }
+}
+
+// Codes and scale byte of a whole block.
+template <int TYPE>
+__device__ __forceinline__ uint32_t quantize_block(const MxPart<TYPE, 32>& v, uint4& q) {
+  float inv;
+  const uint32_t s = mx_scale(v.amax(), inv);
+  uint32_t w[4];
+  v.codes(inv, w);
+  q = make_uint4(w[0], w[1], w[2], w[3]);
+  return s;
 }
 
 // GGUF blocks of 32 values as source (quant.rs:135-190): Q4_0 holds elements
 // 0..15 in the low nibbles and 16..31 in the high ones, offset by 8.
-__device__ __forceinline__ void load_gguf_block(const uint8_t* blk, bool q4, float (&v)[32]) {
+__device__ __forceinline__ void load_gguf_block(const uint8_t* blk, bool q4, MxPart<kF32, 32>& part) {
+  float v[32];
   const uint16_t* h = reinterpret_cast<const uint16_t*>(blk);  // blocks are 2-byte aligned
   const float d = f16_bits_to_f32(h[0]);
   if (q4) {
@@ -50,6 +64,7 @@ __device__ __forceinline__ void load_gguf_block(const uint8_t* blk, bool q4, flo
       v[2 * i + 1] = (float)(int8_t)(w >> 8) * d;
     }
   }
+  memcpy(part.w, v, sizeof(v));
 }
 
 // Writes a block; the four lanes of blocks 4g .. 4g+3 of a row (adjacent
@@ -85,7 +100,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const void* __restric
   } else {
     row = tile * kMxRows + r;
   }
-  float v[32];
+  constexpr int kPart = TYPE < 0 ? kF32 : TYPE;
+  MxPart<kPart, 32> v;
   if (row < rows && b * 32 < cols) {
     if constexpr (TYPE >= 0) {
       using T = typename Elem<TYPE>::T;
@@ -95,18 +111,19 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const void* __restric
                       q4 != 0, v);
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    v.zero();
   }
   uint4 q;
-  const uint32_t s = mx_quantize32(v, q);
+  const uint32_t s = quantize_block(v, q);
   store_block(dst + ((size_t)m * tiles + tile) * mx_tile_bytes(nb), nb, r, b, q, s, b < nb);
 }
 
 // Both directions in one read: a CTA stages 64 rows x 128 columns in shared
-// memory; each thread then quantises one block along a row and one along a
-// column (a block of the transposed matrix).  `dst` [rows][cols] and `dst_t`
-// [cols][rows] are written with whole 128-byte lines.
+// memory; a thread then quantises one block along a row, and one along a
+// column (a block of the transposed matrix) together with a partner: each of
+// the two reads 16 rows of two adjacent columns, so that 16-bit values come in
+// whole words, they share the columns' maxima, and one half block of codes
+// changes hands.  Both outputs are written in whole 128-byte lines.
 constexpr int kBothRows = 64, kBothCols = 128;
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_quantize_both_kernel(const typename Elem<TYPE>::T* __restrict__ src,
@@ -121,91 +138,147 @@ __global__ void __launch_bounds__(256) mx4_quantize_both_kernel(const typename E
   pdl_trigger();
   const int nx = (cols + kMxRows - 1) / kMxRows * (kMxRows / kBothCols);  // every row of dst_t's tiles
   const int r0 = blockIdx.x / nx * kBothRows, c0 = blockIdx.x % nx * kBothCols;
-  for (int i = threadIdx.x; i < kBothRows * (kBothCols / E::kVec); i += 256) {
-    const int r = i / (kBothCols / E::kVec), c = (i % (kBothCols / E::kVec)) * E::kVec;
+  constexpr int kVecs = kBothCols / E::kVec, kLoads = kBothRows * kVecs / 256;
+  uint4 u[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = (threadIdx.x + 256 * i) / kVecs, c = (threadIdx.x % kVecs) * E::kVec;
     const T* p = src + (r0 + r) * ldx + c0 + c;
-    uint4 u = make_uint4(0, 0, 0, 0);
+    u[i] = make_uint4(0, 0, 0, 0);
     if (r0 + r < rows) {
       if (vec && c0 + c + E::kVec <= cols) {
-        u = __ldg(reinterpret_cast<const uint4*>(p));
+        u[i] = __ldg(reinterpret_cast<const uint4*>(p));
       } else {
         T t[E::kVec];
 #pragma unroll
         for (int j = 0; j < E::kVec; ++j) t[j] = c0 + c + j < cols ? p[j] : E::put(0.f);
-        memcpy(&u, t, 16);
+        memcpy(&u[i], t, 16);
       }
     }
-    *reinterpret_cast<uint4*>(&sm[r * kPitch + c]) = u;
   }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    *reinterpret_cast<uint4*>(&sm[(threadIdx.x + 256 * i) / kVecs * kPitch + (threadIdx.x % kVecs) * E::kVec]) = u[i];
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float v[32];
-  uint4 q;
   {
     const int r = warp * 8 + (lane >> 2), b = lane & 3, nb = mx_blocks(cols);
-    const uint4* p = reinterpret_cast<const uint4*>(&sm[r * kPitch + b * 32]);
-#pragma unroll
-    for (int i = 0; i < 32 / E::kVec; ++i) E::unpack(p[i], v + i * E::kVec);
-    const uint32_t s = mx_quantize32(v, q);
+    MxPart<TYPE, 32> v;
+    memcpy(v.w, __builtin_assume_aligned(&sm[r * kPitch + b * 32], 16), sizeof(v.w));
+    uint4 q;
+    const uint32_t s = quantize_block(v, q);
     const int row = r0 + r, bg = (c0 >> 5) + b;
     store_block(dst + (size_t)(row / kMxRows) * mx_tile_bytes(nb), nb, row % kMxRows, bg, q, s, bg < nb);
   }
   {
-    // 16 columns x 2 blocks per warp: a block of 8 columns is one line
-    const int c = warp * 16 + (lane & 15), b = lane >> 4, nb = mx_blocks(rows);
+    // 32 columns x 1 block per warp: lanes l and l + 16 take rows 0..15 and
+    // 16..31 of columns 2l and 2l + 1
+    const int half = lane >> 4, c = (warp & 3) * 32 + (lane & 15) * 2, b = warp >> 2, nb = mx_blocks(rows);
+    const T* p = &sm[(b * 32 + half * 16) * kPitch + c];
+    MxPart<TYPE, 16> x, y;
+    if constexpr (TYPE == kF32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = E::get(sm[(b * 32 + i) * kPitch + c]);
-    const uint32_t s = mx_quantize32(v, q);
-    const int row = c0 + c, bg = (r0 >> 5) + b;
+      for (int i = 0; i < 16; ++i) {
+        uint2 t;
+        memcpy(&t, __builtin_assume_aligned(p + i * kPitch, 8), 8);
+        x.w[i] = t.x, y.w[i] = t.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t t0, t1;
+        memcpy(&t0, __builtin_assume_aligned(p + 2 * i * kPitch, 4), 4);
+        memcpy(&t1, __builtin_assume_aligned(p + (2 * i + 1) * kPitch, 4), 4);
+        x.w[i] = __byte_perm(t0, t1, 0x5410);
+        y.w[i] = __byte_perm(t0, t1, 0x7632);
+      }
+    }
+    uint32_t mx = x.amax(), my = y.amax();
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+    my = max(my, __shfl_xor_sync(0xffffffffu, my, 16));
+    float ix, iy;
+    const uint32_t sx = mx_scale(mx, ix), sy = mx_scale(my, iy);
+    uint32_t qx[2], qy[2];
+    x.codes(ix, qx);
+    y.codes(iy, qy);
+    // the lower lane ends with all of column 2l, the upper with 2l + 1
+    const uint32_t g0 = __shfl_xor_sync(0xffffffffu, half ? qx[0] : qy[0], 16);
+    const uint32_t g1 = __shfl_xor_sync(0xffffffffu, half ? qx[1] : qy[1], 16);
+    const uint4 q = half ? make_uint4(g0, g1, qy[0], qy[1]) : make_uint4(qx[0], qx[1], g0, g1);
+    const int row = c0 + c + half, bg = (r0 >> 5) + b;
     if (bg < nb) {
       uint8_t* tile = dst_t + (size_t)(row / kMxRows) * mx_tile_bytes(nb);
       *reinterpret_cast<uint4*>(tile + mx_code_offset(nb, row % kMxRows, bg)) = q;
-      tile[mx_scale_offset(row % kMxRows, bg)] = (uint8_t)s;
+      tile[mx_scale_offset(row % kMxRows, bg)] = (uint8_t)(half ? sy : sx);
     }
   }
 }
 
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  // magnitude codes 0..7 -> 0, .5, 1, 1.5, 2, 3, 4, 6
-  const uint32_t m = code & 7u, ex = m >> 1, f = m & 1u;
-  const float a = ex ? __uint_as_float(((ex + 126u) << 23) | (f << 22)) : 0.5f * f;
-  return code & 8u ? -a : a;
+// Two E2M1 codes (a byte) as f32.
+__device__ __forceinline__ float2 e2m1_pair(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 a;\n\tcvt.u8.u32 a, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(byte));
+  __half2 v;
+  memcpy(&v, &h, 4);
+  return __half22float2(v);
 }
 
-// A lane takes 8 values (4 code bytes); 16 lanes write 128 contiguous values
-// of a row.
+// A warp takes 8 rows x 128 columns of a tile: lanes side by side write one
+// 16-byte vector each of a row, and the addresses of the first rows serve all
+// eight.  (The codes of the 8 rows are four lines, read once and then from
+// L1.)
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t* __restrict__ src,
                                                              typename Elem<TYPE>::T* __restrict__ dst, long long ldo,
                                                              long long mstride, int rows, int cols, int gated,
                                                              int vec) {
   using E = Elem<TYPE>;
+  constexpr int V = E::kVec, kLanes = 128 / V, kStep = 32 / kLanes;  // lanes per row, rows at a time
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nx = (cols + 127) / 128, m = blockIdx.y;
-  const int row = blockIdx.x / nx * 16 + warp * 2 + (lane >> 4);
-  const int c0 = blockIdx.x % nx * 128 + (lane & 15) * 8, b = c0 >> 5;
-  if (row >= rows || c0 >= cols) return;
-  const int nb = mx_blocks(cols), tiles = (rows + kMxRows - 1) / kMxRows;
-  int tile = row / kMxRows, r = row % kMxRows;
-  if (gated) mx_gated_row(rows, row, tile, r);
+  const int tiles = (rows + kMxRows - 1) / kMxRows, tile = (int)(blockIdx.x / nx) >> 1;
+  const int g = ((int)(blockIdx.x / nx) & 1) * 8 + warp;  // row group of the tile
+  const int c = (int)(blockIdx.x % nx) * 128 + (lane % kLanes) * V, b = c >> 5;
+  if (c >= cols) return;
+  const int nb = mx_blocks(cols), r0 = g * 8 + lane / kLanes;
   const uint8_t* t = src + ((size_t)m * tiles + tile) * mx_tile_bytes(nb);
-  const uint32_t q = *reinterpret_cast<const uint32_t*>(t + mx_code_offset(nb, r, b) + (lane & 3) * 4);
-  const uint32_t s = t[mx_scale_offset(r, b)];
-  // 2^(s - 127); s = 0 is the subnormal 2^-127, s = 255 NaN
-  const float scale = s == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(s ? s << 23 : 0x00400000u);
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = e2m1_value(q >> (4 * i)) * scale;
-  typename E::T* o = dst + m * mstride + row * ldo + c0;
-  if (vec && c0 + 8 <= cols) {
-#pragma unroll
-    for (int i = 0; i < 8 / E::kVec; ++i) reinterpret_cast<uint4*>(o)[i] = E::pack(v + i * E::kVec);
+  const uint8_t* qp = t + mx_code_offset(nb, r0, b) + (c & 31) / 2;
+  const uint8_t* sp = t + mx_scale_offset(r0, b);
+  int row, limit;  // of the first row, and where the rows end
+  if (gated) {
+    const int I = rows >> 1;
+    row = tile * 64 + (r0 & 63) + (r0 < 64 ? 0 : I);
+    limit = r0 < 64 ? I : rows;
   } else {
+    row = tile * kMxRows + r0;
+    limit = rows;
+  }
+  typename E::T* o = dst + m * mstride + row * ldo + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c0 + i < cols) o[i] = E::put(v[i]);
+  for (int i = 0; i < 8; i += kStep) {
+    if (row + i >= limit) break;
+    uint32_t q;
+    if constexpr (V == 8) q = __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * i));
+    else q = __ldg(reinterpret_cast<const uint16_t*>(qp + 16 * i));
+    const uint32_t s = __ldg(sp + 16 * i);
+    // 2^(s - 127); s = 0 is the subnormal 2^-127, s = 255 NaN
+    const float scale = s == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(s ? s << 23 : 0x00400000u);
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      const float2 f = e2m1_pair((q >> (8 * j)) & 0xffu);
+      v[2 * j] = f.x * scale, v[2 * j + 1] = f.y * scale;
+    }
+    if (vec && c + V <= cols) {
+      *reinterpret_cast<uint4*>(o) = E::pack(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < cols) o[j] = E::put(v[j]);
+    }
+    o += kStep * ldo;
   }
 }
 
@@ -222,15 +295,11 @@ __global__ void __launch_bounds__(256) mx4_gather_kernel(const typename Elem<TYP
   const long long i = (long long)blockIdx.x * 8 + warp;
   const int t = (int)(i / spans), b = (int)(i % spans) * 32 + lane;
   if (t >= T) return;
-  float v[32];
-  if (b * 32 < H) {
-    load_block<TYPE>(x + t * ldx, b, H, vec != 0, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-  }
+  MxPart<TYPE, 32> v;
+  if (b * 32 < H) load_block<TYPE>(x + t * ldx, b, H, vec != 0, v);
+  else v.zero();
   uint4 q;
-  uint32_t s = mx_quantize32(v, q);
+  const uint32_t s = quantize_block(v, q);
   uint32_t w = s << (8 * (b & 3));
   w |= __shfl_xor_sync(0xffffffffu, w, 1);
   w |= __shfl_xor_sync(0xffffffffu, w, 2);
@@ -244,6 +313,53 @@ __global__ void __launch_bounds__(256) mx4_gather_kernel(const typename Elem<TYP
     *reinterpret_cast<uint4*>(tile + mx_code_offset(nb, at % kMxRows, b)) = q;
     if ((b & 3) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(at % kMxRows, b)) = w;
   }
+}
+
+// The same in two steps for large batches, where the 16-byte stores above,
+// each half a 32-byte sector in a line of eight different tokens, are what
+// bounds: the tokens quantised once, row by row (codes [T][nb][16], scales
+// [T][nb / 2 * 2 rounded to 4]), then whole lines gathered.
+__host__ __device__ inline int flat_scales(int nb) { return (nb + 3) & ~3; }
+
+template <int TYPE>
+__global__ void __launch_bounds__(256) mx4_quantize_flat_kernel(const typename Elem<TYPE>::T* __restrict__ x,
+                                                                long long ldx, uint4* __restrict__ codes,
+                                                                uint8_t* __restrict__ scales, int T, int H, int vec) {
+  pdl_wait();
+  pdl_trigger();
+  const int nb = mx_blocks(H), np = flat_scales(nb);
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int t = (int)(i / np), b = (int)(i % np);
+  if (t >= T) return;
+  MxPart<TYPE, 32> v;
+  if (b * 32 < H) load_block<TYPE>(x + t * ldx, b, H, vec != 0, v);
+  else v.zero();
+  uint4 q;
+  scales[i] = (uint8_t)quantize_block(v, q);
+  if (b < nb) codes[(size_t)t * nb + b] = q;
+}
+
+// A warp takes 8 positions (a row group): lane = (row, block of four).
+__global__ void __launch_bounds__(256) mx4_gather_flat_kernel(const uint4* __restrict__ codes,
+                                                              const uint8_t* __restrict__ scales,
+                                                              const int32_t* __restrict__ pair,
+                                                              const int32_t* __restrict__ end,
+                                                              uint8_t* __restrict__ dst, int H, int K, int n_rows) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const int row = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 8 + (lane >> 2);
+  if (row >= min(n_rows, __ldg(end))) return;
+  const int p = __ldg(pair + row);
+  if (p < 0) return;
+  const int nb = mx_blocks(H), r = row % kMxRows;
+  const uint4* q = codes + (size_t)(p / K) * nb;
+  const uint32_t* s = reinterpret_cast<const uint32_t*>(scales + (size_t)(p / K) * flat_scales(nb));
+  uint8_t* tile = dst + (size_t)(row / kMxRows) * mx_tile_bytes(nb);
+#pragma unroll 4
+  for (int b = j; b < nb; b += 4) *reinterpret_cast<uint4*>(tile + mx_code_offset(nb, r, b)) = __ldg(q + b);
+  for (int g = j; g < (nb + 3) / 4; g += 4)
+    *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, 4 * g)) = __ldg(s + g);
 }
 
 bool vec_ok(const void* p, long long ld, long long mstride, size_t s) {
@@ -280,7 +396,7 @@ cudaError_t launch_mx4_quantize_both(int type, const void* x, long long ldx, uin
 
 cudaError_t launch_mx4_dequantize(int type, const uint8_t* src, void* out, long long ldo, long long mstride, int rows,
                                   int cols, int matrices, bool gated, cudaStream_t s) {
-  const dim3 grid((unsigned)((cols + 127) / 128 * (long long)((rows + 15) / 16)), matrices);
+  const dim3 grid((unsigned)((cols + 127) / 128 * (long long)((rows + kMxRows - 1) / kMxRows * 2)), matrices);
   const int vec = vec_ok(out, ldo, mstride, elem_bytes(type)), g = gated;
   switch (type) {
     case kF32: return launch_pdl(mx4_dequantize_kernel<kF32>, grid, 256, 0, s, src, (float*)out, ldo, mstride, rows, cols, g, vec);
@@ -289,15 +405,40 @@ cudaError_t launch_mx4_dequantize(int type, const uint8_t* src, void* out, long 
   }
 }
 
-cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int32_t* pos, uint8_t* dst, int T, int H,
-                              int K, cudaStream_t s) {
-  const int spans = (mx_blocks(H) + 31) / 32;
-  const dim3 grid((unsigned)(((long long)T * spans + 7) / 8));
-  const int vec = vec_ok(x, ldx, 0, elem_bytes(type));
+// Pairs from which the gather runs in two steps.
+constexpr long long kGatherFlatPairs = 8192;
+
+size_t mx4_flat_bytes(int H, int K, int T) {
+  const int nb = mx_blocks(H);
+  return (long long)T * K < kGatherFlatPairs ? 0 : (size_t)T * (nb * 16 + flat_scales(nb));
+}
+
+namespace {
+template <int TYPE>
+cudaError_t gather_as(const void* x, long long ldx, const int32_t* pos, const int32_t* pair, const int32_t* end,
+                      uint8_t* dst, uint8_t* flat, int T, int H, int K, int n_rows, cudaStream_t s) {
+  using E = typename Elem<TYPE>::T;
+  const int vec = vec_ok(x, ldx, 0, sizeof(E)), nb = mx_blocks(H);
+  if ((long long)T * K < kGatherFlatPairs) {
+    const dim3 grid((unsigned)(((long long)T * ((nb + 31) / 32) + 7) / 8));
+    return launch_pdl(mx4_gather_kernel<TYPE>, grid, 256, 0, s, (const E*)x, ldx, pos, dst, T, H, K, vec);
+  }
+  uint4* codes = reinterpret_cast<uint4*>(flat);
+  uint8_t* scales = flat + (size_t)T * nb * 16;
+  const dim3 grid((unsigned)(((long long)T * flat_scales(nb) + 255) / 256));
+  const cudaError_t st = launch_pdl(mx4_quantize_flat_kernel<TYPE>, grid, 256, 0, s, (const E*)x, ldx, codes, scales, T, H, vec);
+  if (st != cudaSuccess) return st;
+  return launch_pdl(mx4_gather_flat_kernel, dim3((n_rows + 63) / 64), 256, 0, s, (const uint4*)codes, (const uint8_t*)scales, pair, end, dst, H, K, n_rows);
+}
+}  // namespace
+
+cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int32_t* pos, const int32_t* pair,
+                              const int32_t* end, uint8_t* dst, uint8_t* flat, int T, int H, int K, int n_rows,
+                              cudaStream_t s) {
   switch (type) {
-    case kF32: return launch_pdl(mx4_gather_kernel<kF32>, grid, 256, 0, s, (const float*)x, ldx, pos, dst, T, H, K, vec);
-    case kF16: return launch_pdl(mx4_gather_kernel<kF16>, grid, 256, 0, s, (const __half*)x, ldx, pos, dst, T, H, K, vec);
-    default: return launch_pdl(mx4_gather_kernel<kBF16>, grid, 256, 0, s, (const __nv_bfloat16*)x, ldx, pos, dst, T, H, K, vec);
+    case kF32: return gather_as<kF32>(x, ldx, pos, pair, end, dst, flat, T, H, K, n_rows, s);
+    case kF16: return gather_as<kF16>(x, ldx, pos, pair, end, dst, flat, T, H, K, n_rows, s);
+    default: return gather_as<kBF16>(x, ldx, pos, pair, end, dst, flat, T, H, K, n_rows, s);
   }
 }
 

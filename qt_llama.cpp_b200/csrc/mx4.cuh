@@ -62,19 +62,22 @@ __host__ __device__ inline void mx_gated_row(int rows, int row, int& tile, int& 
   r = (i & 63) + (up << 6);
 }
 
-// Eight E2M1 codes of v * inv (inv a power of two), the first in the lowest
-// nibble.  The conversion rounds to nearest even and saturates at 6.
-__device__ __forceinline__ uint32_t mx_pack8(const float* v, float inv) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t b;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
-        : "=r"(b)
-        : "f"(v[2 * i + 1] * inv), "f"(v[2 * i] * inv));
-    r |= b << (8 * i);
-  }
+// Eight E2M1 codes, the first in the lowest nibble.  The conversion rounds to
+// nearest even and saturates at 6.
+__device__ __forceinline__ uint32_t mx_codes8(float v0, float v1, float v2, float v3, float v4, float v5, float v6,
+                                              float v7) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v0), "f"(v1), "f"(v2), "f"(v3), "f"(v4), "f"(v5), "f"(v6), "f"(v7));
   return r;
+}
+// ... of v * inv, inv a power of two.
+__device__ __forceinline__ uint32_t mx_pack8(const float* v, float inv) {
+  return mx_codes8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
 }
 
 // Scale byte of a block whose largest |v| has the bits `amax` (as an unsigned
@@ -89,17 +92,6 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t amax, float& inv) {
   const int e = ex - 2 > 0 ? ex - 2 : 0;  // e + 127
   inv = __uint_as_float((uint32_t)(254 - e) << 23);
   return (uint32_t)e;
-}
-
-// Quantises 32 values: four words of codes and the scale byte.
-__device__ __forceinline__ uint32_t mx_quantize32(const float (&v)[32], uint4& q) {
-  uint32_t amax = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-  float inv;
-  const uint32_t s = mx_scale(amax, inv);
-  q = make_uint4(mx_pack8(v, inv), mx_pack8(v + 8, inv), mx_pack8(v + 16, inv), mx_pack8(v + 24, inv));
-  return s;
 }
 
 // Element types: 16-byte vectors to and from f32.
@@ -163,6 +155,48 @@ struct Elem<kBF16> {
       memcpy(&w[i], &h, 4);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// N values of a block held as they came: f32, or pairs of 16-bit floats, whose
+// magnitudes are compared two at a time as integers (they order alike, NaN
+// above infinity).
+template <int TYPE, int N>
+struct MxPart {
+  static constexpr int kWords = TYPE == kF32 ? N : N / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // Bits of the largest magnitude, as f32.
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
+    if constexpr (TYPE == kF32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      m = max(m & 0xffffu, m >> 16);
+      if constexpr (TYPE == kBF16) return m << 16;
+      else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) & 0x7fffffffu;
+    }
+  }
+  // Codes of the values times inv, eight to a word.
+  __device__ __forceinline__ void codes(float inv, uint32_t* q) const {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      float v[8];
+      if constexpr (TYPE == kF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[8 * i + j]);
+      } else {
+        Elem<TYPE>::unpack(make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]), v);
+      }
+      q[i] = mx_pack8(v, inv);
+    }
   }
 };
 

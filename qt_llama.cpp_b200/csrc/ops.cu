@@ -71,6 +71,7 @@ struct ExpertsWs {
   SortWs sort;
   int32_t *offsets, *counts, *pos, *pair;
   uint8_t *x, *act;  // MXFP4 rows in expert order: tokens [H], activations [I]
+  uint8_t* flat;     // the tokens quantised row by row (large batches)
   float* y;          // down products [row][H]
   int n_rows;
   size_t bytes;
@@ -92,6 +93,7 @@ ExpertsWs carve_experts(void* base, int H, int I, int E, int K, int T) {
   w.pair = reinterpret_cast<int32_t*>(take((size_t)w.n_rows * 4));
   w.x = take(mrml::mx_matrix_bytes(w.n_rows, H));
   w.act = take(mrml::mx_matrix_bytes(w.n_rows, I));
+  w.flat = take(mrml::mx4_flat_bytes(H, K, T));
   w.y = reinterpret_cast<float*>(take((size_t)w.n_rows * H * 4));
   w.bytes = off;
   return w;
@@ -102,7 +104,7 @@ int check_product(int type, int M, int N, int K) {
   if (!is_float(type)) return MRML_ERR_UNSUPPORTED;
   if (M < 0 || N <= 0 || K <= 0) return MRML_ERR_INVALID_ARGUMENT;
   if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00) return MRML_ERR_UNSUPPORTED;
-  if (((long long)M + 127) / 128 * (((long long)N + 127) / 128) > 0x7fffffffll) return MRML_ERR_UNSUPPORTED;
+  if (((long long)M + 127) / 128 * (((long long)N + 127) / 128) > (1ll << 30)) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
 }
 
@@ -298,7 +300,7 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
   const long long tiles = w.n_rows / mrml::kMxRows + 1;
   MRML_LAUNCH(mrml::launch_sort(ids, w.offsets, w.counts, w.pos, w.pair, E, T * K, mrml::kMxRows, w.n_rows,
                                 w.sort.chunk_cnt, w.sort.status, s));
-  MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.x, T, H, K, s));
+  MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.pair, w.offsets + E, w.x, w.flat, T, H, K, w.n_rows, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, gate_up, w.x, w.offsets, w.counts, E, 0, 2 * I, H, true, nullptr, 0,
                                     w.act, tiles, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H,

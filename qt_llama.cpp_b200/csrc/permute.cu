@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
                                                         int H, int K, int per_token) {
   using EI = Elem<TYPE_IN>;
   using E = Elem<TYPE>;
-  constexpr int V = VEC ? 8 : 1;  // values per thread
+  constexpr int V = VEC ? EI::kVec : 1;  // values per thread: one 16-byte load of a row
   pdl_wait();
   pdl_trigger();
   const long long t = blockIdx.x / per_token;
@@ -203,21 +203,17 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
       if (scale && at[j] >= 0) w[j] *= __ldg(scale + __ldg(ids + t * K + k0 + j));
     }
     if constexpr (VEC) {
-      constexpr int N = 8 / EI::kVec;
-      uint4 u[8][N];
+      uint4 u[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (at[j] >= 0) u[j][n] = __ldg(reinterpret_cast<const uint4*>(rows + (size_t)at[j] * H + c) + n);
+        if (at[j] >= 0) u[j] = __ldg(reinterpret_cast<const uint4*>(rows + (size_t)at[j] * H + c));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (at[j] < 0) continue;
-        float v[8];
+        float v[V];
+        EI::unpack(u[j], v);
 #pragma unroll
-        for (int n = 0; n < N; ++n) EI::unpack(u[j][n], v + n * EI::kVec);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], v[i], acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(w[j], v[i], acc[i]);
       }
     } else {
 #pragma unroll
@@ -227,8 +223,10 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
   }
   typename E::T* o = out + t * ldo + c;
   if constexpr (VEC) {
+    typename E::T r[V];
 #pragma unroll
-    for (int n = 0; n < 8 / E::kVec; ++n) reinterpret_cast<uint4*>(o)[n] = E::pack(acc + n * E::kVec);
+    for (int i = 0; i < V; ++i) r[i] = E::put(acc[i]);
+    memcpy(__builtin_assume_aligned(o, V * sizeof(r[0])), r, sizeof(r));
   } else {
     *o = E::put(acc[0]);
   }
@@ -359,8 +357,8 @@ cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* prob
                          const float* scale, void* out, long long ldo, int H, int K, int T, cudaStream_t s) {
   using I = typename Elem<TI>::T;
   using O = typename Elem<TO>::T;
-  const bool vec = H % 8 == 0 && rows_aligned(rows, H, sizeof(I)) && rows_aligned(out, ldo, sizeof(O));
-  const int per = (H + 128 * (vec ? 8 : 1) - 1) / (128 * (vec ? 8 : 1));
+  const bool vec = rows_aligned(rows, H, sizeof(I)) && rows_aligned(out, ldo, sizeof(O));
+  const int v = vec ? Elem<TI>::kVec : 1, per = (H + 128 * v - 1) / (128 * v);
   const dim3 grid((unsigned)((long long)T * per)), block(128);
   return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per)
              : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per);
