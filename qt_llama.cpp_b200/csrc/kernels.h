@@ -198,7 +198,8 @@ cudaError_t launch_ep_combine_push(uint8_t* const* slabs, int rank, int N, int T
 cudaError_t launch_ep_reduce(uint8_t* const* slabs, int rank, int N, int T, int H, int E, int K, const int32_t* ids,
                              const float* probs, float* out, int* err, cudaStream_t s);
 // (token, slot) pairs sorted by expert, rows gathered and brought back
-// (permute.cu).  sort_chunk_ints: ints of scratch for large sorts.
+// (permute.cu).  sort_chunk_ints: ints of scratch for large sorts; pair may be
+// null.
 size_t sort_chunk_ints(long long n_pairs, int E);
 cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, int32_t* pos, int32_t* pair, int E,
                         int n_pairs, int align, int n_rows, int32_t* chunk_cnt, int* err, cudaStream_t s);

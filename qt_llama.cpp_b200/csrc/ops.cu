@@ -298,8 +298,8 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
   const ExpertsWs w = carve_experts(workspace, H, I, E, K, T);
   const cudaStream_t s = (cudaStream_t)stream;
   const long long tiles = w.n_rows / mrml::kMxRows + 1;
-  MRML_LAUNCH(mrml::launch_sort(ids, w.offsets, w.counts, w.pos, w.pair, E, T * K, mrml::kMxRows, w.n_rows,
-                                w.sort.chunk_cnt, w.sort.status, s));
+  MRML_LAUNCH(mrml::launch_sort(ids, w.offsets, w.counts, w.pos, mrml::mx4_flat_bytes(H, K, T) ? w.pair : nullptr,
+                                E, T * K, mrml::kMxRows, w.n_rows, w.sort.chunk_cnt, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.pair, w.offsets + E, w.x, w.flat, T, H, K, w.n_rows, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, gate_up, w.x, w.offsets, w.counts, E, 0, 2 * I, H, true, nullptr, 0,
                                     w.act, tiles, w.sort.status, s));

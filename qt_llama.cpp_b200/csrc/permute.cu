@@ -28,11 +28,24 @@ struct SortArgs {
   int n_pairs, E, align, n_rows, chunk;
 };
 
+// Every row starts without a pair.
+__device__ __forceinline__ void clear_pairs(const SortArgs& a) {
+  if (!a.pair) return;
+  const int stride = gridDim.x * blockDim.x;
+  int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (((uintptr_t)a.pair & 15) == 0) {
+    for (; r < a.n_rows / 4; r += stride) reinterpret_cast<int4*>(a.pair)[r] = make_int4(-1, -1, -1, -1);
+    r = (a.n_rows & ~3) + blockIdx.x * blockDim.x + threadIdx.x;
+  }
+  for (; r < a.n_rows; r += stride) a.pair[r] = -1;
+}
+
 __global__ void __launch_bounds__(1024) sort_count_kernel(SortArgs a) {
   __shared__ int cnt[kMaxExperts];
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) cnt[e] = 0;
   pdl_wait();
   pdl_trigger();
+  clear_pairs(a);
   __syncthreads();
   const int p0 = blockIdx.x * a.chunk, p1 = min(a.n_pairs, p0 + a.chunk);
   for (int p = p0 + threadIdx.x; p < p1; p += blockDim.x) {
@@ -54,6 +67,7 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
   for (int i = threadIdx.x; i < nw * E + 2 * E; i += blockDim.x) sm[i] = 0;
   pdl_wait();
   pdl_trigger();
+  if (gridDim.x == 1) clear_pairs(a);
   __syncthreads();
   int e[ITEMS], rank[ITEMS];
   const int p0 = blockIdx.x * a.chunk + warp * 32 * ITEMS;
@@ -86,24 +100,32 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
     if (gridDim.x == 1) tot[x] = s;
   }
   if (gridDim.x > 1) {
-    // this chunk's start and the totals, from every chunk's counts
-    for (int i = threadIdx.x; i < (int)gridDim.x * E; i += blockDim.x) {
-      const int c = a.chunk_cnt[i], x = i % E;
-      if (c) {
-        atomicAdd(&tot[x], c);
-        if (i / E < (int)blockIdx.x) atomicAdd(&before[x], c);
+    // this chunk's start and the totals, from every chunk's counts: a thread
+    // sums one expert over every (threads / E)-th chunk
+    const int x = threadIdx.x % E, step = blockDim.x / E, chunks = gridDim.x;
+    if ((int)threadIdx.x < step * E) {
+      int all = 0, mine = 0;
+#pragma unroll 8
+      for (int c = threadIdx.x / E; c < chunks; c += step) {
+        const int n = __ldg(a.chunk_cnt + (size_t)c * E + x);
+        all += n;
+        if (c < (int)blockIdx.x) mine += n;
       }
+      atomicAdd(&tot[x], all);
+      atomicAdd(&before[x], mine);
     }
   }
   __syncthreads();
-  if (warp == 0) {  // aligned starts: each lane scans E / 32 experts
+  for (int x = threadIdx.x; x < E; x += blockDim.x) off[x] = (tot[x] + a.align - 1) / a.align * a.align;
+  __syncthreads();
+  if (warp == 0) {  // starts: each lane scans the rows of E / 32 experts
     constexpr int kPer = kMaxExperts / 32;
     int c[kPer], s = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int x = lane * kPer + i;
       c[i] = s;
-      if (x < E) s += (tot[x] + a.align - 1) / a.align * a.align;
+      if (x < E) s += off[x];
     }
     int up = s;
 #pragma unroll
@@ -124,15 +146,11 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
       int at = -1;
       if (e[i] >= 0) {
         at = off[e[i]] + before[e[i]] + wcnt[warp * E + e[i]] + rank[i];
-        a.pair[at] = p;
+        if (a.pair) a.pair[at] = p;
       }
       a.pos[p] = at;
     }
   }
-  // rows that no pair takes
-  for (int x = blockIdx.x; x < E; x += gridDim.x)
-    for (int r = off[x] + tot[x] + threadIdx.x; r < off[x + 1]; r += blockDim.x) a.pair[r] = -1;
-  for (int r = off[E] + blockIdx.x * blockDim.x + threadIdx.x; r < a.n_rows; r += gridDim.x * blockDim.x) a.pair[r] = -1;
   if (blockIdx.x == 0) {
     for (int x = threadIdx.x; x < E; x += blockDim.x) a.counts[x] = tot[x];
     for (int x = threadIdx.x; x <= E; x += blockDim.x) a.offsets[x] = off[x];
@@ -323,8 +341,9 @@ cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, i
                         int n_pairs, int align, int n_rows, int32_t* chunk_cnt, int* err, cudaStream_t s) {
   SortArgs a{ids, offsets, counts, pos, pair, chunk_cnt, err, n_pairs, E, align, n_rows, 0};
   const bool one = n_pairs <= kSortOne;
-  const int items = one ? (n_pairs <= 1024 ? 1 : 4) : sort_chunk(n_pairs) / 1024;
-  const int threads = one ? std::min(1024, std::max(256, (n_pairs + 31) / 32 * 32)) : 1024;
+  // one CTA: few warps, whose counts are scanned one after another
+  const int items = one ? (n_pairs <= 256 ? 1 : 4) : sort_chunk(n_pairs) / 1024;
+  const int threads = one ? (n_pairs <= 1024 ? 256 : 1024) : 1024;
   a.chunk = items * threads;
   const int grid = std::max(1, (n_pairs + a.chunk - 1) / a.chunk);
   const size_t smem = (size_t)(threads / 32 * E + 3 * E + 1) * 4;

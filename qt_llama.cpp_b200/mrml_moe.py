@@ -410,30 +410,44 @@ def quantize(wtype, src, dst, stream=None):
 # contiguous columns; their row strides are taken from the tensors).
 
 
-def _float_type(t) -> int:
-    import torch
+_torch_types = None
 
-    types = {torch.float32: MRML_F32, torch.float16: MRML_F16, torch.bfloat16: MRML_BF16}
-    assert t.dtype in types, f"unsupported element type {t.dtype}"
-    return types[t.dtype]
+
+def _types():
+    """(element types by dtype, int32, float32), torch being imported only when tensors come in."""
+    global _torch_types
+    if _torch_types is None:
+        import torch
+
+        _torch_types = ({torch.float32: MRML_F32, torch.float16: MRML_F16, torch.bfloat16: MRML_BF16}, torch.int32,
+                        torch.float32)
+    return _torch_types
+
+
+def _float_type(t) -> int:
+    ty = (_torch_types or _types())[0].get(t.dtype)
+    assert ty is not None, f"unsupported element type {t.dtype}"
+    return ty
 
 
 def _ld(t) -> int:
     """Row stride in elements of a tensor whose last axis is contiguous."""
+    if t.is_contiguous():
+        return t.shape[-1]
     assert t.stride(-1) == 1 or t.shape[-1] == 1, "columns must be contiguous"
     return t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]
 
 
 def _check_ints(*tensors):
-    import torch
-
-    assert all(t is None or (t.dtype == torch.int32 and t.is_contiguous()) for t in tensors), "int32, contiguous"
+    i32 = (_torch_types or _types())[1]
+    for t in tensors:
+        assert t is None or (t.dtype == i32 and t.is_contiguous()), "int32, contiguous"
 
 
 def _check_f32(*tensors):
-    import torch
-
-    assert all(t is None or (t.dtype == torch.float32 and t.is_contiguous()) for t in tensors), "f32, contiguous"
+    f32 = (_torch_types or _types())[2]
+    for t in tensors:
+        assert t is None or (t.dtype == f32 and t.is_contiguous()), "f32, contiguous"
 
 
 def _zeroed(nbytes: int, device):
@@ -446,6 +460,8 @@ def _zeroed(nbytes: int, device):
 
 def sorted_rows(E, K, T, align=1) -> int:
     """Rows of the sorted order (an upper bound when align > 1)."""
+    if align == 1 and E > 0 and K > 0 and 0 <= T * K <= 1 << 30:
+        return T * K
     n = load_library().mrml_moe_sorted_rows(E, K, T, align)
     if n < 0:
         raise MoeError("mrml_moe_sorted_rows", n, "invalid argument")
@@ -527,9 +543,7 @@ def new_mx4(rows, cols, matrices=1, device=None):
 
 
 def _check_mx4(q, rows, cols, matrices=1):
-    import torch
-
-    assert q.dtype == torch.uint8 and q.is_contiguous() and q.numel() >= mx4_bytes(rows, cols, matrices)
+    assert q.element_size() == 1 and q.is_contiguous() and q.numel() >= mx4_bytes(rows, cols, matrices)
 
 
 def mx4_quantize(src, dst, rows, cols, matrices=1, gated=False, wtype=None, stream=None):
