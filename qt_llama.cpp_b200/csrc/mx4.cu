@@ -118,13 +118,15 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const void* __restric
   store_block(dst + ((size_t)m * tiles + tile) * mx_tile_bytes(nb), nb, r, b, q, s, b < nb);
 }
 
-// Both directions in one read: a CTA stages 64 rows x 128 columns in shared
-// memory; a thread then quantises one block along a row, and one along a
+// Both directions in one read: a CTA stages 64 (f32) or 128 rows x 128 columns
+// in shared memory; a thread then quantises blocks along a row, and blocks along a
 // column (a block of the transposed matrix) together with a partner: each of
-// the two reads 16 rows of two adjacent columns, so that 16-bit values come in
-// whole words, they share the columns' maxima, and one half block of codes
-// changes hands.  Both outputs are written in whole 128-byte lines.
-constexpr int kBothRows = 64, kBothCols = 128;
+// the two reads half the rows of two adjacent columns, so that 16-bit values
+// come in whole words, they share the columns' maxima, and half a block of
+// codes changes hands.  Both outputs are written in whole 128-byte lines.
+constexpr int kBothCols = 128;
+template <int TYPE>
+constexpr int kBothRows = TYPE == kF32 ? 64 : 128;  // of 48 KB of shared memory
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_quantize_both_kernel(const typename Elem<TYPE>::T* __restrict__ src,
                                                                 long long ldx, uint8_t* __restrict__ dst,
@@ -132,84 +134,120 @@ __global__ void __launch_bounds__(256) mx4_quantize_both_kernel(const typename E
                                                                 int vec) {
   using E = Elem<TYPE>;
   using T = typename E::T;
-  constexpr int kPitch = kBothCols + 16 / sizeof(T);  // 16-byte aligned rows, shifted by four banks each
-  __shared__ __align__(16) T sm[kBothRows * kPitch];
+  constexpr int kRows = kBothRows<TYPE>, kIter = kRows / 64;
+  // Rows are shifted by eight banks each.  Along a row, lanes of the upper two
+  // blocks read their 16-byte pieces with neighbours exchanged; along the
+  // columns the two lanes of a pair take rows 4j, 4j + 1 and 4j + 2, 4j + 3:
+  // both without bank conflicts for 16-bit values.
+  constexpr int kPitch = kBothCols + 32 / sizeof(T);
+  __shared__ __align__(16) T sm[kRows * kPitch];
   pdl_wait();
   pdl_trigger();
   const int nx = (cols + kMxRows - 1) / kMxRows * (kMxRows / kBothCols);  // every row of dst_t's tiles
-  const int r0 = blockIdx.x / nx * kBothRows, c0 = blockIdx.x % nx * kBothCols;
-  constexpr int kVecs = kBothCols / E::kVec, kLoads = kBothRows * kVecs / 256;
-  uint4 u[kLoads];
+  const int r0 = blockIdx.x / nx * kRows, c0 = blockIdx.x % nx * kBothCols;
+  constexpr int kVecs = kBothCols / E::kVec, kLoads = kRows * kVecs / 256;
+  const int lr = threadIdx.x / kVecs, lc = (threadIdx.x % kVecs) * E::kVec;
+  {
+    const T* p = src + (r0 + lr) * ldx + c0 + lc;
+    uint4 u[kLoads];
+    if (vec && r0 + kRows <= rows && c0 + kBothCols <= cols) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = (threadIdx.x + 256 * i) / kVecs, c = (threadIdx.x % kVecs) * E::kVec;
-    const T* p = src + (r0 + r) * ldx + c0 + c;
-    u[i] = make_uint4(0, 0, 0, 0);
-    if (r0 + r < rows) {
-      if (vec && c0 + c + E::kVec <= cols) {
-        u[i] = __ldg(reinterpret_cast<const uint4*>(p));
-      } else {
+      for (int i = 0; i < kLoads; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p + i * (256 / kVecs) * ldx));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const T* q = p + i * (256 / kVecs) * ldx;
         T t[E::kVec];
 #pragma unroll
-        for (int j = 0; j < E::kVec; ++j) t[j] = c0 + c + j < cols ? p[j] : E::put(0.f);
+        for (int j = 0; j < E::kVec; ++j)
+          t[j] = r0 + lr + i * (256 / kVecs) < rows && c0 + lc + j < cols ? q[j] : E::put(0.f);
         memcpy(&u[i], t, 16);
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
-    *reinterpret_cast<uint4*>(&sm[(threadIdx.x + 256 * i) / kVecs * kPitch + (threadIdx.x % kVecs) * E::kVec]) = u[i];
+    for (int i = 0; i < kLoads; ++i)
+      *reinterpret_cast<uint4*>(&sm[(lr + i * (256 / kVecs)) * kPitch + lc]) = u[i];
+  }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   {
-    const int r = warp * 8 + (lane >> 2), b = lane & 3, nb = mx_blocks(cols);
-    MxPart<TYPE, 32> v;
-    memcpy(v.w, __builtin_assume_aligned(&sm[r * kPitch + b * 32], 16), sizeof(v.w));
-    uint4 q;
-    const uint32_t s = quantize_block(v, q);
-    const int row = r0 + r, bg = (c0 >> 5) + b;
-    store_block(dst + (size_t)(row / kMxRows) * mx_tile_bytes(nb), nb, row % kMxRows, bg, q, s, bg < nb);
-  }
-  {
-    // 32 columns x 1 block per warp: lanes l and l + 16 take rows 0..15 and
-    // 16..31 of columns 2l and 2l + 1
-    const int half = lane >> 4, c = (warp & 3) * 32 + (lane & 15) * 2, b = warp >> 2, nb = mx_blocks(rows);
-    const T* p = &sm[(b * 32 + half * 16) * kPitch + c];
-    MxPart<TYPE, 16> x, y;
-    if constexpr (TYPE == kF32) {
+    const int r = warp * 8 + (lane >> 2), b = lane & 3, nb = mx_blocks(cols), bg = (c0 >> 5) + b;
+    uint8_t* tile = dst + (size_t)(r0 / kMxRows) * mx_tile_bytes(nb);
+    const int rt = r0 % kMxRows + r, n = min(kMxChunk, nb - bg / kMxChunk * kMxChunk);
+    uint8_t* qp = tile + mx_code_offset(nb, rt, bg);
+    uint8_t* sp = tile + mx_scale_offset(rt, bg);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        uint2 t;
-        memcpy(&t, __builtin_assume_aligned(p + i * kPitch, 8), 8);
-        x.w[i] = t.x, y.w[i] = t.y;
+    for (int i = 0; i < kIter; ++i) {  // 64 rows further: 8 row groups, two words of scales
+      MxPart<TYPE, 32> v;
+      const int swap = (b >> 1) * E::kVec;
+#pragma unroll
+      for (int k = 0; k < 32 / E::kVec; ++k)
+        memcpy(v.w + 4 * k, __builtin_assume_aligned(&sm[(r + 64 * i) * kPitch + b * 32 + (k * E::kVec ^ swap)], 16), 16);
+      uint4 q;
+      uint32_t w = quantize_block(v, q) << (8 * b);
+      if (swap) {  // 8 codes per 16-byte piece of 16-bit values, 4 of f32
+        if constexpr (TYPE == kF32) {
+          q = make_uint4(__byte_perm(q.x, 0, 0x1032), __byte_perm(q.y, 0, 0x1032), __byte_perm(q.z, 0, 0x1032),
+                         __byte_perm(q.w, 0, 0x1032));
+        } else {
+          q = make_uint4(q.y, q.x, q.w, q.z);
+        }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t t0, t1;
-        memcpy(&t0, __builtin_assume_aligned(p + 2 * i * kPitch, 4), 4);
-        memcpy(&t1, __builtin_assume_aligned(p + (2 * i + 1) * kPitch, 4), 4);
-        x.w[i] = __byte_perm(t0, t1, 0x5410);
-        y.w[i] = __byte_perm(t0, t1, 0x7632);
+      w |= __shfl_xor_sync(0xffffffffu, w, 1);
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      if (bg < nb) {
+        *reinterpret_cast<uint4*>(qp + i * 8 * (n * 128)) = q;
+        if (b == 0) *reinterpret_cast<uint32_t*>(sp + 8 * i) = w;
       }
     }
-    uint32_t mx = x.amax(), my = y.amax();
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-    my = max(my, __shfl_xor_sync(0xffffffffu, my, 16));
-    float ix, iy;
-    const uint32_t sx = mx_scale(mx, ix), sy = mx_scale(my, iy);
-    uint32_t qx[2], qy[2];
-    x.codes(ix, qx);
-    y.codes(iy, qy);
-    // the lower lane ends with all of column 2l, the upper with 2l + 1
-    const uint32_t g0 = __shfl_xor_sync(0xffffffffu, half ? qx[0] : qy[0], 16);
-    const uint32_t g1 = __shfl_xor_sync(0xffffffffu, half ? qx[1] : qy[1], 16);
-    const uint4 q = half ? make_uint4(g0, g1, qy[0], qy[1]) : make_uint4(qx[0], qx[1], g0, g1);
-    const int row = c0 + c + half, bg = (r0 >> 5) + b;
-    if (bg < nb) {
-      uint8_t* tile = dst_t + (size_t)(row / kMxRows) * mx_tile_bytes(nb);
-      *reinterpret_cast<uint4*>(tile + mx_code_offset(nb, row % kMxRows, bg)) = q;
-      tile[mx_scale_offset(row % kMxRows, bg)] = (uint8_t)(half ? sy : sx);
+  }
+  {
+    // 32 columns x 1 block per warp: lanes l and l + 16 each take 16 of the
+    // block's rows in columns 2l and 2l + 1
+    const int half = lane >> 4, c = (warp & 3) * 32 + (lane & 15) * 2, nb = mx_blocks(rows);
+    const int row = c0 + c + half, bg = (r0 >> 5) + (warp >> 2);
+    const T* p = &sm[((warp >> 2) * 32 + half * 2) * kPitch + c];
+    uint8_t* tile = dst_t + (size_t)(row / kMxRows) * mx_tile_bytes(nb);
+    uint8_t* qp = tile + mx_code_offset(nb, row % kMxRows, bg);
+    uint8_t* sp = tile + mx_scale_offset(row % kMxRows, bg);
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {  // two blocks further, in the same chunk (r0 is a multiple of 128 then)
+      MxPart<TYPE, 16> x, y;
+      if constexpr (TYPE == kF32) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          uint2 t;
+          memcpy(&t, __builtin_assume_aligned(p + (64 * i + j / 2 * 4 + j % 2) * kPitch, 8), 8);
+          x.w[j] = t.x, y.w[j] = t.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t t0, t1;
+          memcpy(&t0, __builtin_assume_aligned(p + (64 * i + 4 * j) * kPitch, 4), 4);
+          memcpy(&t1, __builtin_assume_aligned(p + (64 * i + 4 * j + 1) * kPitch, 4), 4);
+          x.w[j] = __byte_perm(t0, t1, 0x5410);
+          y.w[j] = __byte_perm(t0, t1, 0x7632);
+        }
+      }
+      uint32_t mx = x.amax(), my = y.amax();
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      my = max(my, __shfl_xor_sync(0xffffffffu, my, 16));
+      float ix, iy;
+      const uint32_t sx = mx_scale(mx, ix), sy = mx_scale(my, iy);
+      uint32_t qx[2], qy[2];
+      x.codes(ix, qx);
+      y.codes(iy, qy);
+      // the lower lane ends with all of column 2l, the upper with 2l + 1; a
+      // byte holds two rows, so the lanes' bytes alternate
+      const uint32_t g0 = __shfl_xor_sync(0xffffffffu, half ? qx[0] : qy[0], 16);
+      const uint32_t g1 = __shfl_xor_sync(0xffffffffu, half ? qx[1] : qy[1], 16);
+      const uint32_t l0 = half ? g0 : qx[0], l1 = half ? g1 : qx[1], u0 = half ? qy[0] : g0, u1 = half ? qy[1] : g1;
+      if (bg + 2 * i < nb) {
+        *reinterpret_cast<uint4*>(qp + 256 * i) = make_uint4(__byte_perm(l0, u0, 0x5140), __byte_perm(l0, u0, 0x7362),
+                                                             __byte_perm(l1, u1, 0x5140), __byte_perm(l1, u1, 0x7362));
+        sp[2 * i] = (uint8_t)(half ? sy : sx);
+      }
     }
   }
 }
@@ -385,7 +423,7 @@ cudaError_t launch_mx4_quantize_both(int type, const void* x, long long ldx, uin
                                      int cols, cudaStream_t s) {
   // every row of both matrices' tiles, so that the padding is written too
   const int pr = (rows + kMxRows - 1) / kMxRows * kMxRows, pc = (cols + kMxRows - 1) / kMxRows * kMxRows;
-  const dim3 grid((unsigned)((long long)(pc / kBothCols) * (pr / kBothRows)));
+  const dim3 grid((unsigned)((long long)(pc / kBothCols) * (pr / (type == kF32 ? kBothRows<kF32> : kBothRows<kBF16>))));
   const int vec = vec_ok(x, ldx, 0, elem_bytes(type));
   switch (type) {
     case kF32: return launch_pdl(mx4_quantize_both_kernel<kF32>, grid, 256, 0, s, (const float*)x, ldx, dst, dst_t, rows, cols, vec);

@@ -177,8 +177,13 @@ struct MxPart {
       for (int i = 0; i < N; ++i) m = max(m, w[i] & 0x7fffffffu);
       return m;
     } else {
+      // one instruction per pair: the larger magnitude, NaN if either is
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (TYPE == kBF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+        else asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+      }
+      m &= 0x7fff7fffu;
       m = max(m & 0xffffu, m >> 16);
       if constexpr (TYPE == kBF16) return m << 16;
       else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) & 0x7fffffffu;
@@ -192,10 +197,19 @@ struct MxPart {
       if constexpr (TYPE == kF32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[8 * i + j]);
+        q[i] = mx_pack8(v, inv);
+      } else if constexpr (TYPE == kBF16) {
+        // scaled in pairs: exact, but for values so small that their code is 0
+        const uint32_t inv2 = __byte_perm(__float_as_uint(inv), 0, 0x3232);
+        uint32_t t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(t[j]) : "r"(w[4 * i + j]), "r"(inv2));
+        Elem<TYPE>::unpack(make_uint4(t[0], t[1], t[2], t[3]), v);
+        q[i] = mx_codes8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
       } else {
         Elem<TYPE>::unpack(make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]), v);
+        q[i] = mx_pack8(v, inv);
       }
-      q[i] = mx_pack8(v, inv);
     }
   }
 };
