@@ -14,11 +14,21 @@
 //
 // A work unit is (expert, 128 weight rows, 128 token rows).  One persistent
 // CTA per SM takes units in turn:
-//   warp 0     producer: one bulk copy per operand and K chunk (the matrix
-//              format is the shared-memory operand layout, mx4.cuh)
-//   warp 1     TMEM allocation; lane 0 copies the chunk's scales to tensor
+//   warps 0, 2 producers of the weights and of the tokens: a bulk copy per K
+//              chunk (the matrix format is the shared-memory operand layout,
+//              mx4.cuh)
+//   warp 1     TMEM allocation; one lane copies the chunk's scales to tensor
 //              memory and issues the MMAs
 //   warps 4-11 epilogue, on the other of two accumulators
+//
+// With many tokens per expert those units are bound by the copies from L2 to
+// shared memory: 34 KB per 128 x 128 x 256 step at the 64 bytes a cycle that
+// an SM takes in is twice the tensor cores' time.  There, pairs of CTAs share
+// a unit of 256 weight rows and 192 token rows (cta_group::2, M = 256): each
+// copies its own 128 weight rows and half of the token rows, 31 KB per 128 x
+// 192 x 256, and the first CTA's warp 1 issues for both.  The second CTA's
+// warp 1 passes on that its stage has landed.
+//
 // Scales live in tensor memory per shared-memory stage, so a stage's scales
 // are overwritten only after the MMAs that read them have completed.
 // Every wait is bounded; on a timeout the CTA records the error, drains its
@@ -39,12 +49,24 @@ using tc::tmem_wait_ld;
 using tc::wait_bar;
 
 constexpr int kStages = 5;
-constexpr int kStageBytes = 2 * kMxChunkBytes;
 constexpr int kThreads = 384;
 constexpr int kExPitch = 33;                          // f32 per row of the GeGLU exchange
 constexpr int kExBytes = 2 * kMxRows * kExPitch * 4;  // two groups' 128 rows x 32 tokens
-constexpr uint32_t kAcc0 = 0, kAccCols = 128;       // two accumulators of 128 columns
-constexpr uint32_t kSf0 = 256, kSfCols = 16;        // scales: 8 + 8 columns per stage
+
+// Shapes of one CTA (kPair = false) and of a pair.  A stage holds the weights'
+// chunk, then the tokens' scales (one group of 1024 bytes per 128-row tile
+// that the unit touches) and codes.  Tensor memory holds two accumulators,
+// then each stage's scales: 8 columns of weights, then per four blocks one
+// group of four columns per token tile.
+template <bool kPair>
+struct Shape {
+  static constexpr int kTokens = kPair ? 192 : 128;             // token rows of a unit
+  static constexpr int kTokenTiles = kPair ? 2 : 1;             // 128-row tiles they touch
+  static constexpr int kTokenScales = kTokenTiles * 1024;
+  static constexpr int kStageBytes = kMxChunkBytes + kTokenScales + (kPair ? kTokens / 2 : kTokens) * kMxChunk * 16;
+  static constexpr uint32_t kSf0 = 2 * kTokens, kSfCols = 8 + 8 * kTokenTiles;
+  static_assert(kSf0 + kStages * kSfCols <= 512, "tensor memory has 512 columns");
+};
 
 struct Params {
   const uint8_t* w;        // weight tiles [E][w_tiles]
@@ -60,7 +82,7 @@ struct Params {
 };
 
 struct __align__(8) Bars {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint64_t full[kStages], empty[kStages], peer_full[kStages], acc_full[2], acc_empty[2], drain;
   uint32_t tmem_base;
   int abort;
   int first[kMaxExperts + 1];  // token tiles of earlier experts
@@ -79,25 +101,68 @@ __device__ __forceinline__ uint64_t desc(uint32_t lo, uint32_t sbo) {
 }
 
 // Instruction descriptor of kind::mxf4: E2M1 operands (1), both K-major, E8M0
-// scales (bit 23), M = 128; N in bits 17-22 (N / 8), the scales' pair within
-// their 32-bit column in bits 4-5 (B) and 29-30 (A).
-__device__ __forceinline__ uint32_t idesc(int N, int sf) {
-  return (uint32_t)sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | 1u << 23 | (uint32_t)(kMxRows >> 4) << 24 |
+// scales (bit 23), M = 128 or 256; N in bits 17-22 (N / 8), the scales' pair
+// within their 32-bit column in bits 4-5 (B) and 29-30 (A).
+__device__ __forceinline__ uint32_t idesc(int M, int N, int sf) {
+  return (uint32_t)sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | 1u << 23 | (uint32_t)(M >> 4) << 24 |
          (uint32_t)sf << 29;
 }
 
+#define MRML_MMA_MXF4(GROUP)                                                                              \
+  asm volatile(                                                                                           \
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"                                                  \
+      "tcgen05.mma.cta_group::" #GROUP                                                                    \
+      ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),              \
+      "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"((uint32_t)add))
+template <bool kPair>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb,
                                          bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"((uint32_t)add));
+  if constexpr (kPair) MRML_MMA_MXF4(2);
+  else MRML_MMA_MXF4(1);
 }
+#undef MRML_MMA_MXF4
 
 // 32 lanes x 16 bytes of shared memory to four TMEM columns, the same in each
-// of the four lane quarters.
+// of the four lane quarters (in a pair: each CTA's memory to its own TMEM).
+template <bool kPair>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t lo) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(lo, 128)) : "memory");
+  if constexpr (kPair)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(lo, 128)) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc(lo, 128)) : "memory");
+}
+
+// Arrives on a barrier (in a pair: on both CTAs') once the MMAs and copies
+// issued so far have completed.
+template <bool kPair>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (kPair)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    mma_commit(bar);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrives on the first CTA's barrier at the same offset.  What it reports (a
+// stage's copies, an accumulator's reads) has completed by then; no memory of
+// this thread's own is handed over, so the arrival needs no release over the
+// cluster, which took 900 cycles and bounded the pair's chunk rate.
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -128,7 +193,8 @@ __device__ __forceinline__ bool all_of_group(bool ok, int id) {
 __device__ __forceinline__ bool try_at(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -156,6 +222,22 @@ __device__ __forceinline__ void copy_at(uint32_t dst, const void* src, uint32_t 
                : "memory");
 }
 
+// A producer's place in the ring of stages.
+struct Ring {
+  uint32_t empty0, full0, ring0;
+  int s;
+  uint32_t ph;
+  __device__ __forceinline__ uint32_t empty() const { return empty0 + 8 * s; }
+  __device__ __forceinline__ uint32_t full() const { return full0 + 8 * s; }
+  __device__ __forceinline__ uint32_t stage(int bytes) const { return ring0 + s * bytes; }
+  __device__ __forceinline__ void next() {
+    if (++s == kStages) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
 // One lane of a converged warp.  The compiler knows such a branch to have a
 // single thread and keeps the operands of the tensor-core instructions in
 // uniform registers; under `lane == 0` it serialises every one of them over
@@ -167,40 +249,44 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// The units of a CTA in turn (each role walks them by itself): weight tile,
+// The units of a CTA (or pair) in turn (each role walks them by itself): weight tile,
 // first token row, tokens.  Within an expert, units that follow one another
 // share the weight tile.  The expert only moves forward, by steps through
 // shared memory; searching for it in the offsets in global memory cost each
 // role 1000 to 1700 cycles per unit.
+template <bool kPair>
 struct Units {
-  int u, e, first, next;  // unit; expert, its first unit and the next expert's
+  static constexpr int kTokens = Shape<kPair>::kTokens;
+  int u, e, w_units, first, next;  // unit; expert, its first unit and the next expert's
   int wt, row0, n;
   size_t w_tile;
 
   __device__ __forceinline__ void start(const Params& P, const Bars* B) {
-    u = (int)blockIdx.x;
+    u = (int)blockIdx.x / (kPair ? 2 : 1);
+    w_units = kPair ? (P.w_tiles + 1) / 2 : P.w_tiles;
     e = 0;
     first = 0;
-    next = P.offsets ? B->first[1] * P.w_tiles : 0x7fffffff;
+    next = P.offsets ? B->first[1] * w_units : 0x7fffffff;
   }
   __device__ __forceinline__ void locate(const Params& P, const Bars* B) {
     if (P.offsets) {
       while (u >= next) {  // u is below the last expert's end
         ++e;
         first = next;
-        next = B->first[e + 1] * P.w_tiles;
+        next = B->first[e + 1] * w_units;
       }
       const unsigned tt = (unsigned)(B->first[e + 1] - B->first[e]), r = (unsigned)(u - first);
       wt = (int)(r / tt);
       const int t = (int)(r - wt * tt);
-      row0 = B->row0[e] + t * kMxRows;
-      n = min(kMxRows, B->count[e] - t * kMxRows);
+      row0 = B->row0[e] + t * kTokens;
+      n = min(kTokens, B->count[e] - t * kTokens);
     } else {
-      const unsigned tt = (unsigned)(P.n_tokens + kMxRows - 1) / kMxRows;
+      const unsigned tt = (unsigned)(P.n_tokens + kTokens - 1) / kTokens;
       wt = (int)((unsigned)u / tt);
-      row0 = (int)(u - wt * tt) * kMxRows;
-      n = min(kMxRows, P.n_tokens - row0);
+      row0 = (int)(u - wt * tt) * kTokens;
+      n = min(kTokens, P.n_tokens - row0);
     }
+    if constexpr (kPair) wt = 2 * wt + (int)(blockIdx.x & 1);  // the last pair's second tile may not exist
     w_tile = (size_t)e * P.w_tiles + wt;
   }
 };
@@ -213,53 +299,75 @@ __device__ __forceinline__ float geglu(float g, float u) {
   return __fdividef(g, 1.f + __expf(-z2)) * u;
 }
 
+// What the MMAs of a unit have in common.
+struct Issue {
+  uint32_t acc, id0, id2;
+  uint32_t shift;  // column of the unit's first token row within its scales
+  bool two;        // the unit touches two token tiles
+};
+
 // A chunk of n blocks (even): its scales to tensor memory, then n / 2 MMAs.
-// wa, xa: descriptor low words of the weights' and the tokens' chunk.
-template <int n>
-__device__ __forceinline__ void chunk_mma(uint32_t acc, uint32_t wa, uint32_t xa, uint32_t sf, uint32_t id0,
-                                          uint32_t id2, bool add) {
-  constexpr int kGroups = (n + 3) / 4;
+// wa: descriptor low word of the stage; sf: the stage's scale columns.
+template <bool kPair, int n>
+__device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t sf, bool add) {
+  constexpr int kGroups = (n + 3) / 4, kTiles = Shape<kPair>::kTokenTiles;
+  const uint32_t xs = wa + (kMxChunkBytes >> 4);
+  // one tile's scales are directly followed by its codes (mx4.cuh)
+  const uint32_t xa = xs + (kPair ? Shape<kPair>::kTokenScales >> 4 : 32 * kGroups);
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    copy_scales(sf + 4 * g, wa + 32 * g);
-    copy_scales(sf + 8 + 4 * g, xa + 32 * g);
+    copy_scales<kPair>(sf + 4 * g, wa + 32 * g);
+    copy_scales<kPair>(sf + 8 + 4 * kTiles * g, xs + 32 * g);
+    if (kPair && I.two) copy_scales<kPair>(sf + 12 + 4 * kTiles * g, xs + 64 + 32 * g);
   }
 #pragma unroll
   for (int j = 0; j < n / 2; ++j)
-    mma_mxf4(acc, desc(wa + 32 * kGroups + j * 16, n * 128), desc(xa + 32 * kGroups + j * 16, n * 128),
-             j & 1 ? id2 : id0, sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4, add || j > 0);
+    mma_mxf4<kPair>(I.acc, desc(wa + 32 * kGroups + j * 16, n * 128), desc(xa + j * 16, n * 128), j & 1 ? I.id2 : I.id0,
+                    sf + (j >> 1) * 4, sf + 8 + 4 * kTiles * (j >> 1) + (kPair ? I.shift : 0), add || j > 0);
 }
+
+// Tokens per expert from which pairs of CTAs are used.
+constexpr int kPairTokens = 192;
 
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
 
-template <int MODE>
+template <int MODE, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
+  using S = Shape<kPair>;
+  constexpr int kStageBytes = S::kStageBytes;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Bars* B = reinterpret_cast<Bars*>(smem_raw);
   uint8_t* ring = smem_raw + kBarBytes;
   float* ex = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // GeGLU exchange
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? (int)(blockIdx.x & 1) : 0;  // in the cluster of two
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&B->full[i], 1);
+      mbar_init(&B->full[i], 2);
       mbar_init(&B->empty[i], 1);
+      mbar_init(&B->peer_full[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B->acc_full[i], 1);
-      mbar_init(&B->acc_empty[i], 8);
+      mbar_init(&B->acc_empty[i], kPair ? 16 : 8);
     }
     mbar_init(&B->drain, 1);
     B->abort = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem_base)));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem_base)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem_base)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   pdl_wait();
   pdl_trigger();
-  if (P.offsets && warp == 2) {  // token tiles before each expert
+  if (P.offsets && warp == 3) {  // token tiles before each expert
     constexpr int kPer = kMaxExperts / 32;
     int c[kPer], s = 0;
 #pragma unroll
@@ -270,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
         const int n = P.counts[x];
         B->count[x] = n;
         B->row0[x] = P.offsets[x];
-        s += (n + kMxRows - 1) / kMxRows;
+        s += (n + S::kTokens - 1) / S::kTokens;
       }
     }
     int up = s;
@@ -285,10 +393,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     if (lane == 31) B->first[P.E] = up;
   }
   fence_before();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync();  // both CTAs' barriers are initialised
+  else __syncthreads();
   fence_after();
   const uint32_t tmem = B->tmem_base;
-  const int n_units = (P.offsets ? B->first[P.E] : (P.n_tokens + kMxRows - 1) / kMxRows) * P.w_tiles;
+  const int n_units = (P.offsets ? B->first[P.E] : (P.n_tokens + S::kTokens - 1) / S::kTokens) *
+                      (kPair ? (P.w_tiles + 1) / 2 : P.w_tiles);
+  const int step = (int)gridDim.x / (kPair ? 2 : 1);
   const size_t tile_bytes = mx_tile_bytes(P.nb);
 
   // The producer's and the issuer's loops run in one thread each, where every
@@ -296,82 +407,123 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   // computed, and whole chunks have constant sizes.
   const int n_full = P.nb / kMxChunk, n_tail = P.nb % kMxChunk;
   const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(&B->full[0]), empty0 = smem_u32(&B->empty[0]);
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     if (elect_one()) {
-      int s = 0, issued = 0;
-      uint32_t ph = 0;
-      auto load = [&](const uint8_t* w, const uint8_t* x, uint32_t wb, uint32_t xb) {
-        if (!wait_at(empty0 + 8 * s, ph ^ 1, B, P.err)) return false;
-        const uint32_t bar = full0 + 8 * s, dst = ring0 + s * kStageBytes;
-        expect_at(bar, wb + xb);
-        copy_at(dst, w, wb, bar);
-        copy_at(dst + kMxChunkBytes, x, xb, bar);
-        ++issued;
-        if (++s == kStages) {
-          s = 0;
-          ph ^= 1;
-        }
-        return true;
-      };
+      // Warp 0 copies the weights, warp 2 the tokens: one thread for both was
+      // what bounded the pairs' chunks (up to five copies each).
+      Ring R{empty0, full0, ring0, 0, 0};
+      int issued = 0;
       bool ok = true;
-      Units U;
-      for (U.start(P, B); U.u < n_units && ok; U.u += gridDim.x) {
+      Units<kPair> U;
+      for (U.start(P, B); U.u < n_units && ok; U.u += step) {
         U.locate(P, B);
-        const uint8_t* w = P.w + U.w_tile * tile_bytes;
-        const uint8_t* x = P.x + (size_t)(U.row0 / kMxRows) * tile_bytes;
-        const uint32_t groups = ((U.n + 15) & ~15) >> 3, xb = 1024 + groups * (kMxChunk * 128);
-        for (int c = 0; c < n_full && ok; ++c) {
-          ok = load(w, x, kMxChunkBytes, xb);
-          w += kMxChunkBytes;
-          x += kMxChunkBytes;
+        if (warp == 0) {
+          const bool some = !kPair || U.wt < P.w_tiles;
+          const uint8_t* w = P.w + U.w_tile * tile_bytes;
+          auto load = [&](int n, uint32_t bytes) {
+            if (!(ok = wait_at(R.empty(), R.ph ^ 1, B, P.err))) return;
+            expect_at(R.full(), some ? bytes : 0);
+            if (some) copy_at(R.stage(kStageBytes), w, bytes, R.full());
+            w += kMxChunkBytes;
+            R.next();
+            ++issued;
+          };
+          for (int c = 0; c < n_full && ok; ++c) load(kMxChunk, kMxChunkBytes);
+          if (n_tail && ok) load(n_tail, mx_chunk_bytes(n_tail));
+        } else {
+          const uint8_t* x = P.x + (size_t)(U.row0 / kMxRows) * tile_bytes;
+          const int N = (U.n + 15) & ~15;
+          // the CTA's row groups: all, or in a pair half of them, which may
+          // start in either tile (group gi) and continue in the next (g1 more)
+          const int groups = N / (kPair ? 16 : 8), from = U.row0 % kMxRows / 8 + rank * groups;
+          const int gi = from % 16, g0 = min(groups, 16 - gi), g1 = groups - g0;
+          const bool two = kPair && U.row0 % kMxRows + N > kMxRows;
+          auto load = [&](int n, uint32_t sb) {
+            if (!(ok = wait_at(R.empty(), R.ph ^ 1, B, P.err))) return;
+            const uint32_t dst = R.stage(kStageBytes) + kMxChunkBytes, line = n * 128;
+            if constexpr (kPair) {
+              const uint8_t* xc = x + sb + (from >= 16 ? tile_bytes : 0);
+              expect_at(R.full(), (two ? 2 * sb : sb) + groups * line);
+              copy_at(dst, x, sb, R.full());
+              copy_at(dst + S::kTokenScales, xc + gi * line, g0 * line, R.full());
+              if (two) copy_at(dst + 1024, x + tile_bytes, sb, R.full());
+              if (g1) copy_at(dst + S::kTokenScales + g0 * line, xc + tile_bytes, g1 * line, R.full());
+            } else {  // scales and codes in one run
+              expect_at(R.full(), sb + groups * line);
+              copy_at(dst, x, sb + groups * line, R.full());
+            }
+            x += kMxChunkBytes;
+            R.next();
+            ++issued;
+          };
+          for (int c = 0; c < n_full && ok; ++c) load(kMxChunk, 1024);
+          if (n_tail && ok) load(n_tail, mx_scale_bytes(n_tail));
         }
-        if (n_tail && ok) ok = load(w, x, mx_chunk_bytes(n_tail), mx_scale_bytes(n_tail) + groups * (n_tail * 128));
       }
       // Whatever happened, every copy lands before the block gives up its
       // shared memory.
       for (int i = 0; i < min(issued, kStages); ++i) {
-        if (--s < 0) {
-          s = kStages - 1;
-          ph ^= 1;
+        if (--R.s < 0) {
+          R.s = kStages - 1;
+          R.ph ^= 1;
         }
-        mbar_wait_bounded(&B->full[s], ph, nullptr);
+        mbar_wait_bounded(&B->full[R.s], R.ph, nullptr);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     if (elect_one()) {
       int s = 0, a = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
-      Units U;
-      for (U.start(P, B); U.u < n_units && ok; U.u += gridDim.x) {
+      Units<kPair> U;
+      for (U.start(P, B); U.u < n_units && ok; U.u += step) {
         U.locate(P, B);
-        const int N = (U.n + 15) & ~15;
-        const uint32_t id0 = idesc(N, 0), id2 = idesc(N, 2);
-        if (!(ok = wait_bar(&B->acc_empty[a], aph ^ 1, B, P.err))) break;
+        const int N = (U.n + 15) & ~15, M = kPair ? 2 * kMxRows : kMxRows;
+        const Issue I{tmem + a * S::kTokens, idesc(M, N, 0), idesc(M, N, 2), (uint32_t)(U.row0 % kMxRows / 32),
+                      U.row0 % kMxRows + N > kMxRows};
+        if (!(ok = wait_at(smem_u32(&B->acc_empty[a]), aph ^ 1, B, P.err))) break;
         fence_after();
-        const uint32_t acc = tmem + kAcc0 + a * kAccCols;
         auto chunk = [&](auto issue, bool add) {
           if (!wait_at(full0 + 8 * s, ph, B, P.err)) return false;
+          if (kPair && !wait_at(smem_u32(&B->peer_full[s]), ph, B, P.err)) return false;
           fence_after();
-          const uint32_t wa = desc_lo(ring0 + s * kStageBytes);
-          issue(acc, wa, wa + (kMxChunkBytes >> 4), tmem + kSf0 + s * kSfCols, id0, id2, add);
-          mma_commit(&B->empty[s]);
+          issue(I, desc_lo(ring0 + s * kStageBytes), tmem + S::kSf0 + s * S::kSfCols, add);
+          commit<kPair>(&B->empty[s]);
           if (++s == kStages) {
             s = 0;
             ph ^= 1;
           }
           return true;
         };
-        for (int c = 0; c < n_full && ok; ++c) ok = chunk(chunk_mma<kMxChunk>, c > 0);
-        if (ok && n_tail == 2) ok = chunk(chunk_mma<2>, n_full > 0);
-        if (ok && n_tail == 4) ok = chunk(chunk_mma<4>, n_full > 0);
-        if (ok && n_tail == 6) ok = chunk(chunk_mma<6>, n_full > 0);
+        for (int c = 0; c < n_full && ok; ++c) ok = chunk(chunk_mma<kPair, kMxChunk>, c > 0);
+        if (ok && n_tail == 2) ok = chunk(chunk_mma<kPair, 2>, n_full > 0);
+        if (ok && n_tail == 4) ok = chunk(chunk_mma<kPair, 4>, n_full > 0);
+        if (ok && n_tail == 6) ok = chunk(chunk_mma<kPair, 6>, n_full > 0);
         if (!ok) break;
-        mma_commit(&B->acc_full[a]);
+        commit<kPair>(&B->acc_full[a]);
         if (a ^= 1; a == 0) aph ^= 1;
       }
-      mma_commit(&B->drain);  // and every MMA ends before the TMEM goes
+      commit<kPair>(&B->drain);  // and every MMA ends before the TMEM goes
       mbar_wait_bounded(&B->drain, 0, nullptr);
+    }
+  } else if (kPair && warp == 1) {
+    // the pair's second CTA: tells the first that a stage has landed here
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      Units<kPair> U;
+      const int chunks = n_full + (n_tail > 0);
+      for (U.start(P, B); U.u < n_units && ok; U.u += step) {
+        for (int c = 0; c < chunks; ++c) {
+          if (!(ok = wait_at(full0 + 8 * s, ph, B, P.err))) break;
+          arrive_leader(&B->peer_full[s]);
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
     }
   } else if (warp >= 4) {
     // Two groups of four warps; a group's warp q reads the lanes 32q..32q+31
@@ -380,8 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     const int q = warp & 3, grp = (warp - 4) >> 2;
     int a = 0;
     uint32_t aph = 0;
-    Units U;
-    for (U.start(P, B); U.u < n_units; U.u += gridDim.x) {
+    Units<kPair> U;
+    for (U.start(P, B); U.u < n_units; U.u += step) {
       U.locate(P, B);
       bool ok = wait_bar(&B->acc_full[a], aph, B, P.err);
       // All lanes leave together; the four warps of a group where they meet
@@ -390,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       else ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + kAcc0 + a * kAccCols;
+      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + a * S::kTokens;
       uint32_t r[32];
       if constexpr (MODE == kModeGated) {
         // 32 tokens at a time: all rows to shared memory (rows 0..63 gate,
@@ -399,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
         float* x = ex + grp * (kMxRows * kExPitch);
         const int half = lane & 1, t = (q & 1) * 16 + (lane >> 1), b = q >> 1, blk = U.wt * 2 + b;
         const float* xg = x + (32 * b + 16 * half) * kExPitch + t;
-        uint8_t* tile = P.act + (size_t)(U.row0 / kMxRows) * mx_tile_bytes(nba);
+        const size_t act_tile = mx_tile_bytes(nba);
         for (int c0 = 32 * grp; c0 < U.n; c0 += 64) {
           tmem_ld32(acc + c0, r);
           tmem_wait_ld();
@@ -417,9 +569,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
           float inv;
           const uint32_t s = mx_scale(amax, inv);
           if (c0 + t < U.n && blk < nba) {
-            *reinterpret_cast<uint2*>(tile + mx_code_offset(nba, c0 + t, blk) + 8 * half) =
+            const int row = U.row0 + c0 + t, rt = row % kMxRows;
+            uint8_t* tile = P.act + (size_t)(row / kMxRows) * act_tile;
+            *reinterpret_cast<uint2*>(tile + mx_code_offset(nba, rt, blk) + 8 * half) =
                 make_uint2(mx_pack8(v, inv), mx_pack8(v + 8, inv));
-            if (half == 0) tile[mx_scale_offset(c0 + t, blk)] = (uint8_t)s;
+            if (half == 0) tile[mx_scale_offset(rt, blk)] = (uint8_t)s;
           }
           group_barrier(1 + grp);
         }
@@ -448,33 +602,63 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B->acc_empty[a]);
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(&B->acc_empty[a]);
+        else arrive_leader(&B->acc_empty[a]);
+      }
       if (a ^= 1; a == 0) aph ^= 1;
     }
   }
   __syncwarp();
   fence_before();
-  __syncthreads();
+  // In a pair, neither CTA leaves before the other's reads and arrivals.
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
-template <int MODE>
-cudaError_t launch(const Params& P, int units, cudaStream_t s) {
+template <int MODE, bool kPair>
+cudaError_t launch(const Params& P, long long units, cudaStream_t s) {
   static SmemOptIn cache;
-  const size_t smem = kBarBytes + kStages * kStageBytes + (MODE == kModeGated ? kExBytes : 0);
-  const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE>, smem, cache);
+  const size_t smem = kBarBytes + kStages * Shape<kPair>::kStageBytes + (MODE == kModeGated ? kExBytes : 0);
+  const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE, kPair>, smem, cache);
   if (st != cudaSuccess) return st;
-  return launch_pdl(mx4_gemm_kernel<MODE>, dim3(std::max(1, std::min(units, tc_num_sms()))), dim3(kThreads), smem, s, P);
+  const int ctas = kPair ? 2 : 1;
+  const int grid = ctas * (int)std::max<long long>(1, std::min<long long>(units, tc_num_sms() / ctas));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {2, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = kPair ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<MODE, kPair>, P);
+}
+
+template <bool kPair>
+cudaError_t launch_mode(int mode, const Params& P, long long units, cudaStream_t s) {
+  switch (mode) {
+    case kModeGated: return launch<kModeGated, kPair>(P, units, s);
+    case kModeF32: return launch<kModeF32, kPair>(P, units, s);
+    case kModeF16: return launch<kModeF16, kPair>(P, units, s);
+    default: return launch<kModeBF16, kPair>(P, units, s);
+  }
 }
 
 }  // namespace mx
 
 cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
                             const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
-                            long long ldo, uint8_t* act, long long max_token_tiles, int* err, cudaStream_t s) {
+                            long long ldo, uint8_t* act, long long tokens, int* err, cudaStream_t s) {
   mx::Params P{};
   P.w = w;
   P.x = x;
@@ -489,13 +673,10 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   P.ldo = ldo;
   P.act = act;
   P.err = err;
-  const int units = (int)std::min<long long>(max_token_tiles * P.w_tiles, 1 << 20);
-  if (gated) return mx::launch<mx::kModeGated>(P, units, s);
-  switch (type) {
-    case kF32: return mx::launch<mx::kModeF32>(P, units, s);
-    case kF16: return mx::launch<mx::kModeF16>(P, units, s);
-    default: return mx::launch<mx::kModeBF16>(P, units, s);
-  }
+  const int mode = gated ? mx::kModeGated : type == kF32 ? mx::kModeF32 : type == kF16 ? mx::kModeF16 : mx::kModeBF16;
+  // Pairs of CTAs from an average of kPairTokens tokens per expert.
+  if (tokens >= (long long)mx::kPairTokens * E) return mx::launch_mode<true>(mode, P, (tokens / 192 + E) * ((P.w_tiles + 1) / 2), s);
+  return mx::launch_mode<false>(mode, P, (tokens / 128 + std::min<long long>(E, tokens)) * P.w_tiles, s);
 }
 
 }  // namespace mrml

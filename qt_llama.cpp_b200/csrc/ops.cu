@@ -103,7 +103,7 @@ ExpertsWs carve_experts(void* base, int H, int I, int E, int K, int T) {
 int check_product(int type, int M, int N, int K) {
   if (!is_float(type)) return MRML_ERR_UNSUPPORTED;
   if (M < 0 || N <= 0 || K <= 0) return MRML_ERR_INVALID_ARGUMENT;
-  if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00) return MRML_ERR_UNSUPPORTED;
+  if (M > 0x7fffff00 || N > 0x7fffff00 || K > (1 << 24)) return MRML_ERR_UNSUPPORTED;  // offsets in a tile fit an int
   if (((long long)M + 127) / 128 * (((long long)N + 127) / 128) > (1ll << 30)) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
 }
@@ -249,7 +249,7 @@ int mrml_moe_mx4_matmul(int type, const uint8_t* a, const uint8_t* b, void* out,
   MRML_TRY(check_workspace(workspace, workspace_bytes, mrml_moe_mx4_matmul_workspace_bytes(M, N, K)));
   MRML_TRY(mrml::check_device());
   const cudaStream_t s = (cudaStream_t)stream;
-  MRML_LAUNCH(mrml::launch_mx4_gemm(type, b, a, nullptr, nullptr, 1, M, N, K, false, out, ldo, nullptr, (M + 127) / 128,
+  MRML_LAUNCH(mrml::launch_mx4_gemm(type, b, a, nullptr, nullptr, 1, M, N, K, false, out, ldo, nullptr, M,
                                     static_cast<int*>(workspace), s));
   return MRML_OK;
 }
@@ -297,14 +297,14 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
   MRML_TRY(mrml::check_device());
   const ExpertsWs w = carve_experts(workspace, H, I, E, K, T);
   const cudaStream_t s = (cudaStream_t)stream;
-  const long long tiles = w.n_rows / mrml::kMxRows + 1;
+  const long long pairs = (long long)T * K;
   MRML_LAUNCH(mrml::launch_sort(ids, w.offsets, w.counts, w.pos, mrml::mx4_flat_bytes(H, K, T) ? w.pair : nullptr,
                                 E, T * K, mrml::kMxRows, w.n_rows, w.sort.chunk_cnt, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.pair, w.offsets + E, w.x, w.flat, T, H, K, w.n_rows, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, gate_up, w.x, w.offsets, w.counts, E, 0, 2 * I, H, true, nullptr, 0,
-                                    w.act, tiles, w.sort.status, s));
+                                    w.act, pairs, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H,
-                                    nullptr, tiles, w.sort.status, s));
+                                    nullptr, pairs, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
   return MRML_OK;
 }

@@ -20,6 +20,7 @@ fallback: without the library or an sm_100 GPU every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -149,12 +150,22 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_current_stream = None
+
+
 def _stream_ptr(stream) -> Optional[int]:
-    if stream is None:
+    """The raw stream; for None torch's current one (without building a
+    torch.cuda.Stream for it, 3 us a call, where torch can be asked for it)."""
+    global _current_stream
+    if stream is not None:
+        return stream.cuda_stream or None
+    if _current_stream is None:
         import torch
 
-        stream = torch.cuda.current_stream()
-    return stream.cuda_stream or None
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _current_stream = ((lambda: raw(torch.cuda.current_device())) if raw is not None
+                           else (lambda: torch.cuda.current_stream().cuda_stream))
+    return _current_stream() or None
 
 
 def workspace_bytes(H: int, I: int, E: int, K: int, T: int) -> int:
@@ -531,6 +542,7 @@ def unpermute_grad(dout, rows, pos, pair, probs, drows, dprobs, H, K, T, stream=
 # ---- MXFP4 matrices: uint8 buffers in the library's own layout.
 
 
+@functools.lru_cache(maxsize=1024)
 def mx4_bytes(rows, cols, matrices=1) -> int:
     return int(load_library().mrml_moe_mx4_bytes(rows, cols, matrices))
 

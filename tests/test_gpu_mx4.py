@@ -232,6 +232,8 @@ def check_product(got, a, b, dtype):
 PRODUCTS = [
     (1, 1, 1), (1, 128, 64), (1, 129, 96), (5, 300, 2816), (16, 64, 32), (17, 257, 300), (128, 128, 256), (129, 130, 704),
     (100, 1000, 1000), (300, 704, 2816), (1, 2816, 4224), (513, 384, 640),
+    # shared by pairs of CTAs: whole and ragged token tiles of 192, odd numbers of weight tiles, every short chunk
+    (192, 128, 64), (193, 129, 96), (384, 640, 320), (400, 257, 448), (575, 300, 1000), (1000, 130, 704), (2000, 900, 512),
 ]
 
 
@@ -370,6 +372,7 @@ LAYERS = [
     (37, 8, 61, 320, 100, 0.3, None), (64, 8, 128, 256, 704, 0.0, None), (200, 4, 8, 1000, 500, 0.05, None),
     (300, 2, 5, 256, 64, 0.0, 3), (9, 4, 8, 96, 33, 1.0, None), (513, 1, 3, 65, 129, 0.0, None),
     (2048, 2, 16, 256, 128, 0.0, None),
+    (700, 4, 8, 416, 352, 0.1, None), (1500, 2, 5, 320, 96, 0.0, 4), (900, 8, 16, 264, 200, 0.2, None),
 ]
 
 
