@@ -79,6 +79,11 @@ struct Params {
   long long ldo;
   uint8_t* act;            // gated: MXFP4 [token row][n_out]
   int* err;
+  // Nothing but the tokens (and, for the GeGLU's result, earlier readers of
+  // act) comes from the kernel right before this one, and that kernel let this
+  // one start only after its own predecessors had completed: then the unit
+  // list and the weights need not wait for it.
+  int early;
 };
 
 struct __align__(8) Bars {
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
   }
-  pdl_wait();
+  if (!P.early) pdl_wait();
   pdl_trigger();
   if (P.offsets && warp == 3) {  // token tiles before each expert
     constexpr int kPer = kMaxExperts / 32;
@@ -411,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     if (elect_one()) {
       // Warp 0 copies the weights, warp 2 the tokens: one thread for both was
       // what bounded the pairs' chunks (up to five copies each).
+      if (warp == 2) pdl_wait();
       Ring R{empty0, full0, ring0, 0, 0};
       int issued = 0;
       bool ok = true;
@@ -530,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     // of tensor memory (weight rows), the groups take 32 columns (tokens) in
     // turn.
     const int q = warp & 3, grp = (warp - 4) >> 2;
+    pdl_wait();
     int a = 0;
     uint32_t aph = 0;
     Units<kPair> U;
@@ -658,8 +665,9 @@ cudaError_t launch_mode(int mode, const Params& P, long long units, cudaStream_t
 
 cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
                             const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
-                            long long ldo, uint8_t* act, long long tokens, int* err, cudaStream_t s) {
+                            long long ldo, uint8_t* act, long long tokens, bool early, int* err, cudaStream_t s) {
   mx::Params P{};
+  P.early = early;
   P.w = w;
   P.x = x;
   P.offsets = offsets;

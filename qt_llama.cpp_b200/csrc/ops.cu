@@ -108,6 +108,21 @@ int check_product(int type, int M, int N, int K) {
   return MRML_OK;
 }
 
+// `early`: a was written by the launch right before, b not (launch_mx4_gemm).
+int matmul(int type, const uint8_t* a, const uint8_t* b, void* out, int64_t ldo, int M, int N, int K, void* workspace,
+           size_t workspace_bytes, bool early, mrml_stream_t stream) {
+  MRML_TRY(check_product(type, M, N, K));
+  if (ldo < N) return MRML_ERR_INVALID_ARGUMENT;
+  if (M == 0) return MRML_OK;
+  if (!a || !b || !out || !aligned16(a) || !aligned16(b) || !elem_aligned(out, type)) return MRML_ERR_INVALID_ARGUMENT;
+  MRML_TRY(check_workspace(workspace, workspace_bytes, mrml_moe_mx4_matmul_workspace_bytes(M, N, K)));
+  MRML_TRY(mrml::check_device());
+  const cudaStream_t s = (cudaStream_t)stream;
+  MRML_LAUNCH(mrml::launch_mx4_gemm(type, b, a, nullptr, nullptr, 1, M, N, K, false, out, ldo, nullptr, M, early,
+                                    static_cast<int*>(workspace), s));
+  return MRML_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -242,16 +257,7 @@ size_t mrml_moe_mx4_matmul_workspace_bytes(int M, int N, int K) {
 
 int mrml_moe_mx4_matmul(int type, const uint8_t* a, const uint8_t* b, void* out, int64_t ldo, int M, int N, int K,
                         void* workspace, size_t workspace_bytes, mrml_stream_t stream) {
-  MRML_TRY(check_product(type, M, N, K));
-  if (ldo < N) return MRML_ERR_INVALID_ARGUMENT;
-  if (M == 0) return MRML_OK;
-  if (!a || !b || !out || !aligned16(a) || !aligned16(b) || !elem_aligned(out, type)) return MRML_ERR_INVALID_ARGUMENT;
-  MRML_TRY(check_workspace(workspace, workspace_bytes, mrml_moe_mx4_matmul_workspace_bytes(M, N, K)));
-  MRML_TRY(mrml::check_device());
-  const cudaStream_t s = (cudaStream_t)stream;
-  MRML_LAUNCH(mrml::launch_mx4_gemm(type, b, a, nullptr, nullptr, 1, M, N, K, false, out, ldo, nullptr, M,
-                                    static_cast<int*>(workspace), s));
-  return MRML_OK;
+  return matmul(type, a, b, out, ldo, M, N, K, workspace, workspace_bytes, false, stream);
 }
 
 size_t mrml_moe_mx4_linear_workspace_bytes(int T, int N, int K) {
@@ -272,7 +278,7 @@ int mrml_moe_mx4_linear(int type, const void* x, int64_t ldx, const uint8_t* w, 
   uint8_t* xq = static_cast<uint8_t*>(workspace) + mm;
   if (!aligned16(w) || !elem_aligned(x, type) || !elem_aligned(out, type)) return MRML_ERR_INVALID_ARGUMENT;
   MRML_TRY(mrml_moe_mx4_quantize(type, x, ldx, 0, xq, T, K, 1, 0, stream));
-  return mrml_moe_mx4_matmul(type, xq, w, out, ldo, T, N, K, workspace, mm, stream);
+  return matmul(type, xq, w, out, ldo, T, N, K, workspace, mm, true, stream);
 }
 
 size_t mrml_moe_mx4_experts_workspace_bytes(int H, int I, int E, int K, int T) {
@@ -302,9 +308,9 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
                                 E, T * K, mrml::kMxRows, w.n_rows, w.sort.chunk_cnt, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gather(type, x, ldx, w.pos, w.pair, w.offsets + E, w.x, w.flat, T, H, K, w.n_rows, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, gate_up, w.x, w.offsets, w.counts, E, 0, 2 * I, H, true, nullptr, 0,
-                                    w.act, pairs, w.sort.status, s));
+                                    w.act, pairs, true, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H,
-                                    nullptr, pairs, w.sort.status, s));
+                                    nullptr, pairs, true, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
   return MRML_OK;
 }

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, l
     const uint4* s = reinterpret_cast<const uint4*>(src);
     uint4* d = reinterpret_cast<uint4*>(dst);
 #pragma unroll 4
-    for (int i = lane; i < nv; i += 32) d[i] = p >= 0 ? __ldg(s + i) : make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < nv; i += 32) __stcs(d + i, p >= 0 ? __ldg(s + i) : make_uint4(0, 0, 0, 0));
   } else {
 #pragma unroll 4
     for (int i = lane; i < H; i += 32) {
