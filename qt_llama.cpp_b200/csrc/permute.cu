@@ -189,9 +189,11 @@ __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, l
 }
 
 // --------------------------------------------------------------- unpermute
-// A thread takes one vector of a token's columns and sums its K rows, all of
-// whose loads it issues first (8 at a time).  The weight of slot k is
-// probs[t,k] (1 without probs) times scale[ids[t,k]] (with scale).
+// A CTA takes a token, or one of several column ranges of it (gridDim.y); a
+// thread sums the K rows in two vectors of columns at a time, all of whose
+// loads (16 for 8 slots) it issues before it needs one.  The rows' places and
+// weights are read once for all columns.  The weight of slot k is probs[t,k]
+// (1 without probs) times scale[ids[t,k]] (with scale).
 template <int TYPE_IN, int TYPE, bool VEC>
 __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE_IN>::T* __restrict__ rows,
                                                         const int32_t* __restrict__ pos,
@@ -199,54 +201,69 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
                                                         const int32_t* __restrict__ ids,
                                                         const float* __restrict__ scale,
                                                         typename Elem<TYPE>::T* __restrict__ out, long long ldo,
-                                                        int H, int K, int per_token) {
+                                                        int H, int K) {
   using EI = Elem<TYPE_IN>;
   using E = Elem<TYPE>;
-  constexpr int V = VEC ? EI::kVec : 1;  // values per thread: one 16-byte load of a row
+  constexpr int V = VEC ? EI::kVec : 1;  // values per vector: one 16-byte load of a row
+  constexpr int S = 8;                   // slots at a time
   pdl_wait();
   pdl_trigger();
-  const long long t = blockIdx.x / per_token;
-  const int c = (blockIdx.x % per_token * 128 + threadIdx.x) * V;
-  if (c >= H) return;
-  float acc[V];
+  const long long t = blockIdx.x;
+  int at[S];
+  float w[S];
+  auto slots = [&](int k0) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  for (int k0 = 0; k0 < K; k0 += 8) {
-    int at[8];
-    float w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < S; ++j) {
       at[j] = k0 + j < K ? __ldg(pos + t * K + k0 + j) : -1;
       w[j] = k0 + j < K && probs ? __ldg(probs + t * K + k0 + j) : 1.f;
       if (scale && at[j] >= 0) w[j] *= __ldg(scale + __ldg(ids + t * K + k0 + j));
     }
-    if constexpr (VEC) {
-      uint4 u[8];
+  };
+  slots(0);
+  const int step = gridDim.y * 128 * V;
+  for (int c = (blockIdx.y * 128 + threadIdx.x) * V; c < H; c += 2 * step) {
+    const bool second = c + step < H;
+    float acc[2][V];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at[j] >= 0) u[j] = __ldg(reinterpret_cast<const uint4*>(rows + (size_t)at[j] * H + c));
+    for (int i = 0; i < V; ++i) acc[0][i] = acc[1][i] = 0.f;
+    for (int k0 = 0; k0 < K; k0 += S) {
+      if (k0 > 0 || K > S) slots(k0);
+      uint4 u[2][S];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < S; ++j) {
         if (at[j] < 0) continue;
-        float v[V];
-        EI::unpack(u[j], v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(w[j], v[i], acc[i]);
+        const typename EI::T* p = rows + (size_t)at[j] * H + c;
+        if constexpr (VEC) {
+          u[0][j] = __ldg(reinterpret_cast<const uint4*>(p));
+          if (second) u[1][j] = __ldg(reinterpret_cast<const uint4*>(p + step));
+        } else {
+          u[0][j].x = __float_as_uint(EI::get(p[0]));
+          if (second) u[1][j].x = __float_as_uint(EI::get(p[step]));
+        }
       }
-    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at[j] >= 0) acc[0] = fmaf(w[j], EI::get(rows[(size_t)at[j] * H + c]), acc[0]);
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !second) break;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+          if (at[j] < 0) continue;
+          float v[V];
+          if constexpr (VEC) EI::unpack(u[h][j], v);
+          else v[0] = __uint_as_float(u[h][j].x);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[h][i] = fmaf(w[j], v[i], acc[h][i]);
+        }
+      }
     }
-  }
-  typename E::T* o = out + t * ldo + c;
-  if constexpr (VEC) {
-    typename E::T r[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = E::put(acc[i]);
-    memcpy(__builtin_assume_aligned(o, V * sizeof(r[0])), r, sizeof(r));
-  } else {
-    *o = E::put(acc[0]);
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && !second) break;
+      typename E::T* o = out + t * ldo + c + h * step;
+      typename E::T r[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = E::put(acc[h][i]);
+      memcpy(__builtin_assume_aligned(o, V * sizeof(r[0])), r, sizeof(r));
+    }
   }
 }
 
@@ -377,10 +394,12 @@ cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* prob
   using I = typename Elem<TI>::T;
   using O = typename Elem<TO>::T;
   const bool vec = rows_aligned(rows, H, sizeof(I)) && rows_aligned(out, ldo, sizeof(O));
-  const int v = vec ? Elem<TI>::kVec : 1, per = (H + 128 * v - 1) / (128 * v);
-  const dim3 grid((unsigned)((long long)T * per)), block(128);
-  return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per)
-             : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K, per);
+  // Column ranges per token: enough CTAs to fill the GPU from few tokens.
+  const int v = vec ? Elem<TI>::kVec : 1, most = (H + 128 * v - 1) / (128 * v);
+  const int parts = std::max(1, std::min(most, 4 * tc_num_sms() / std::max(1, T)));
+  const dim3 grid(T, parts), block(128);
+  return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K)
+             : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K);
 }
 
 template <int TYPE>
