@@ -331,9 +331,6 @@ __device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t 
                     sf + (j >> 1) * 4, sf + 8 + 4 * kTiles * (j >> 1) + (kPair ? I.shift : 0), add || j > 0);
 }
 
-// Tokens per expert from which pairs of CTAs are used.
-constexpr int kPairTokens = 192;
-
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
 
 template <int MODE, bool kPair>
@@ -682,8 +679,15 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   P.act = act;
   P.err = err;
   const int mode = gated ? mx::kModeGated : type == kF32 ? mx::kModeF32 : type == kF16 ? mx::kModeF16 : mx::kModeBF16;
-  // Pairs of CTAs from an average of kPairTokens tokens per expert.
-  if (tokens >= (long long)mx::kPairTokens * E) return mx::launch_mode<true>(mode, P, (tokens / 192 + E) * ((P.w_tiles + 1) / 2), s);
+  // Pairs of CTAs pay where there are enough units for several waves of them,
+  // tokens to fill their tiles, and a sum long enough to be bound by the
+  // operands and not by the results.  Measured, one CTA against pairs: 4096 x
+  // 4224 x 2816 bf16 28.4 / 26.7 us (7 tiles per SM), 8192^3 234 / 200; 2048 x
+  // 4224 x 2816 16.8 / 17.0 (3.6), 1024: 10.5 / 12.8, 256: 6.1 / 7.9; 65536
+  // sorted tokens, gated K = 2816 162 / 155, f32 rows K = 704 158 / 168.
+  const long long tiles = (tokens + 127) / 128 * P.w_tiles;
+  if (tokens >= 192ll * E && 2 * tiles >= 9ll * tc_num_sms() && cols >= 1024)
+    return mx::launch_mode<true>(mode, P, (tokens / 192 + E) * ((P.w_tiles + 1) / 2), s);
   return mx::launch_mode<false>(mode, P, (tokens / 128 + std::min<long long>(E, tokens)) * P.w_tiles, s);
 }
 

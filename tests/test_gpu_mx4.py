@@ -222,18 +222,22 @@ def matmul(moe, x, w, dtype, out=None):
 
 def check_product(got, a, b, dtype):
     """got against a b^T of exact values."""
-    want, mag = a @ b.t(), a.abs() @ b.abs().t()
     steps = -(-a.shape[1] // 64)
-    tol = (steps + 2) * 2.0**-23 * mag
-    tol = tol + UNIT[dtype] * (want.abs() + tol) + 2.0**-24 * (dtype == torch.float16)
-    assert ((got.double() - want).abs() <= tol).all()
+    for r in range(0, a.shape[0], 8192):
+        x, y = a[r:r + 8192], got[r:r + 8192]
+        want, mag = x @ b.t(), x.abs() @ b.abs().t()
+        tol = (steps + 2) * 2.0**-23 * mag
+        tol = tol + UNIT[dtype] * (want.abs() + tol) + 2.0**-24 * (dtype == torch.float16)
+        assert ((y.double() - want).abs() <= tol).all()
 
 
 PRODUCTS = [
     (1, 1, 1), (1, 128, 64), (1, 129, 96), (5, 300, 2816), (16, 64, 32), (17, 257, 300), (128, 128, 256), (129, 130, 704),
     (100, 1000, 1000), (300, 704, 2816), (1, 2816, 4224), (513, 384, 640),
-    # shared by pairs of CTAs: whole and ragged token tiles of 192, odd numbers of weight tiles, every short chunk
+    # large ones are shared by pairs of CTAs: whole and ragged token tiles of 192, odd numbers of weight tiles, short
+    # chunks of every length
     (192, 128, 64), (193, 129, 96), (384, 640, 320), (400, 257, 448), (575, 300, 1000), (1000, 130, 704), (2000, 900, 512),
+    (4000, 3330, 1056), (9001, 1500, 1100), (12300, 1000, 1216), (100000, 130, 1024),
 ]
 
 
@@ -373,6 +377,7 @@ LAYERS = [
     (300, 2, 5, 256, 64, 0.0, 3), (9, 4, 8, 96, 33, 1.0, None), (513, 1, 3, 65, 129, 0.0, None),
     (2048, 2, 16, 256, 128, 0.0, None),
     (700, 4, 8, 416, 352, 0.1, None), (1500, 2, 5, 320, 96, 0.0, 4), (900, 8, 16, 264, 200, 0.2, None),
+    (4100, 4, 8, 1088, 700, 0.1, None), (3000, 8, 7, 1040, 333, 0.0, None),
 ]
 
 
