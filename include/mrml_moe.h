@@ -394,8 +394,8 @@ int mrml_moe_sorted_rows(int E, int K, int T, int align);
  * mrml_moe_sorted_rows(E, K, T, align) (the row's pair, or -1 for padding and
  * past the end).  A negative id marks a slot without an expert; an id of E or
  * more is skipped too and sets MRML_ERR_BAD_EXPERT_ID in the workspace
- * (mrml_moe_device_status).  E <= 256, K <= 64.  Workspace: clear it once
- * with mrml_moe_workspace_init. */
+ * (mrml_moe_device_status).  E <= 256, K <= 64, T*K <= 2^26.  Workspace:
+ * clear it once with mrml_moe_workspace_init. */
 size_t mrml_moe_sort_workspace_bytes(int E, int K, int T);
 int mrml_moe_sort(const int32_t *ids, int32_t *offsets, int32_t *counts, int32_t *pos, int32_t *pair, int E, int K,
                   int T, int align, void *workspace, size_t workspace_bytes, mrml_stream_t stream);

@@ -19,23 +19,26 @@ bool is_float(int type) { return type == MRML_F32 || type == MRML_F16 || type ==
 bool is_gguf(int type) { return type == MRML_Q4_0 || type == MRML_Q8_0; }
 bool elem_aligned(const void* p, int type) { return ((uintptr_t)p & (mrml::elem_bytes(type) - 1)) == 0; }
 
+// The most (token, slot) pairs of a call: every chunk of a large sort sums the
+// counts of all chunks, which beyond this would take longer than the rest.
+constexpr long long kMaxPairs = 1ll << 26;
+
 // Rows of the sorted order, padding included; -1 when the arguments are
-// invalid or the rows do not fit an int.
+// invalid.
 long long rows_bound(int E, int K, int T, int align) {
   if (E <= 0 || K <= 0 || T < 0 || align <= 0 || align > 128) return -1;
   const long long pairs = (long long)T * K;
-  if (pairs > (1ll << 30)) return -1;
-  const long long n = pairs + std::min<long long>(E, pairs) * (align - 1);
-  return n <= 0x7fffffffll ? n : -1;
+  if (pairs > kMaxPairs) return -1;
+  return pairs + std::min<long long>(E, pairs) * (align - 1);
 }
 
 // Shapes of the permutation entry points.
 int check_tokens(int type, int H, int K, int T) {
   if (!is_float(type)) return MRML_ERR_UNSUPPORTED;
   if (H <= 0 || K <= 0 || T < 0) return MRML_ERR_INVALID_ARGUMENT;
-  if (K > kMaxTopK || (long long)T * K > (1ll << 30)) return MRML_ERR_UNSUPPORTED;
-  // one CTA per 128 values of a token
-  if ((long long)T * ((H + 127) / 128) > 0x7fffffffll) return MRML_ERR_UNSUPPORTED;
+  if (K > kMaxTopK || (long long)T * K > kMaxPairs) return MRML_ERR_UNSUPPORTED;
+  // the gather takes a warp per 1024 values of a token
+  if ((long long)T * ((H + 1023) / 1024) > 0x7fffffffll) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
 }
 

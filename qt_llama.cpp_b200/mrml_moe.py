@@ -471,7 +471,7 @@ def _zeroed(nbytes: int, device):
 
 def sorted_rows(E, K, T, align=1) -> int:
     """Rows of the sorted order (an upper bound when align > 1)."""
-    if align == 1 and E > 0 and K > 0 and 0 <= T * K <= 1 << 30:
+    if align == 1 and E > 0 and K > 0 and 0 <= T * K <= 1 << 26:
         return T * K
     n = load_library().mrml_moe_sorted_rows(E, K, T, align)
     if n < 0:

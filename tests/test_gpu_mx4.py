@@ -278,6 +278,19 @@ def test_product_of_wide_scales_and_special_blocks(cuda, moe):
     assert torch.equal(torch.isnan(got), bad)
 
 
+def test_product_offsets_past_32_bits(cuda, moe):
+    """70000 x 32768 results (2.3e9 elements), and 2.2e9 quantised values."""
+    M, N, K = 70000, 32768, 64
+    g = torch.Generator(device=cuda).manual_seed(6)
+    x, w = torch.randn(M, K, generator=g, device=cuda), torch.randn(N, K, generator=g, device=cuda)
+    out = matmul(moe, x, w, torch.bfloat16)
+    at = torch.cat([torch.arange(0, M, 4999, device=cuda), torch.arange(M - 20, M, device=cuda)])
+    check_product(out[at], mx4_values(x[at]), mx4_values(w), torch.bfloat16)
+    q = quantize(moe, out)
+    back = values(moe, q, M, N, dtype=torch.bfloat16)[0]
+    assert same(back[at], mx4_values(out[at]))
+
+
 def test_training_step_products(cuda, moe):
     """y = x w^T, dx = dy w and dw = dy^T x from three pairs of quantisations."""
     T, N, K = 200, 328, 264
@@ -378,6 +391,8 @@ LAYERS = [
     (2048, 2, 16, 256, 128, 0.0, None),
     (700, 4, 8, 416, 352, 0.1, None), (1500, 2, 5, 320, 96, 0.0, 4), (900, 8, 16, 264, 200, 0.2, None),
     (4100, 4, 8, 1088, 700, 0.1, None), (3000, 8, 7, 1040, 333, 0.0, None),
+    # large batches, more than 8 slots
+    (2048, 8, 16, 1024, 64, 0.0, None), (6000, 8, 9, 600, 96, 0.05, None), (1500, 12, 24, 1001, 40, 0.3, None),
 ]
 
 

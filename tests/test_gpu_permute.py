@@ -259,3 +259,24 @@ def test_side_stream_and_graph(cuda, moe):
     assert ((out - x).abs() <= 10 * F32 * x.abs()).all()
     ref = sort_numpy(ids.cpu().numpy(), E, 1, n)
     assert np.array_equal(pair.cpu().numpy(), ref[3])
+
+
+def test_offsets_past_32_bits(cuda, moe):
+    """262144 rows of 8704 16-bit values: 2.28e9 elements, 4.6 GB on each side of the gather."""
+    T, K, E, H = 65536, 4, 16, 8704
+    ids = routing(11, T, K, E)
+    (_, _, pos, pair), _ = run_sort(moe, cuda, ids, E, 1)
+    x = torch.empty(T, H, dtype=torch.bfloat16, device=cuda).normal_(generator=torch.Generator(cuda).manual_seed(1))
+    rows = torch.empty(T * K, H, dtype=torch.bfloat16, device=cuda)
+    moe.permute(x, pair, rows, H, K)
+    at = torch.cat([torch.arange(0, T * K, 977, device=cuda), torch.arange(T * K - 50, T * K, device=cuda)])
+    assert torch.equal(rows[at], x[pair[at].long() // K])
+    out = torch.empty_like(x)
+    moe.unpermute(rows, pos, torch.full((T, K), 0.25, device=cuda), out, H, K, T)
+    assert torch.equal(out, x)  # sums of quarters of one value are exact
+    drows, dprobs = torch.empty_like(rows), torch.empty(T, K, device=cuda)
+    moe.unpermute_grad(x, rows, pos, pair, torch.full((T, K), 0.5, device=cuda), drows, dprobs, H, K, T)
+    assert torch.equal(drows[at], 0.5 * x[pair[at].long() // K])
+    t = torch.tensor([0, 1, T // 2, T - 1], device=cuda)
+    sq = x[t].double().square().sum(1)
+    assert ((dprobs[t].double() - sq[:, None]).abs() <= (H + 1) * F32 * sq[:, None]).all()

@@ -64,7 +64,7 @@ def test_permutation_refusals(moe):
         assert fn(0, P, None, P, 64, 64, 2, 4, None) == -1
         assert fn(0, P, P, ODD, 64, 64, 2, 4, None) == -1
         assert fn(0, P, P, P, 64, 64, 2, -4, None) == -1
-        assert fn(0, P, P, P, 1 << 20, 1 << 20, 2, 1 << 20, None) == -2
+        assert fn(0, P, P, P, 64, 64, 2, 1 << 26, None) == -2
         assert fn(0, None, None, None, 64, 64, 2, 0, None) == 0
     grad = lib.mrml_moe_unpermute_grad
     assert grad(0, P, 64, P, P, P, P, P, P, 64, 2, 4, 7, None) == -1  # fewer rows than pairs
