@@ -240,6 +240,11 @@ cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int3
 cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
                             const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
                             long long ldo, uint8_t* act, long long tokens, bool early, int* err, cudaStream_t s);
+// The quantisation of a few tokens x and their product with w in one launch
+// (where mx4_few_tokens says so); results as of the two.
+bool mx4_few_tokens(int tokens, int cols);
+cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long ldx, int n_tokens, int rows, int cols,
+                           void* out, long long ldo, int* err, cudaStream_t s);
 int gate_up_tok_chunk(int wtype, int H);
 int down_tok_chunk(int wtype, int I);
 

@@ -10,37 +10,6 @@ namespace mrml {
 
 namespace {
 
-// The 32 values of block b of a row that starts at `row`; zero past `cols`.
-template <int TYPE>
-__device__ __forceinline__ void load_block(const typename Elem<TYPE>::T* row, int b, int cols, bool vec,
-                                           MxPart<TYPE, 32>& v) {
-  const int c0 = b * 32;
-  if (vec && c0 + 32 <= cols) {
-    const uint4* p = reinterpret_cast<const uint4*>(row + c0);
-#pragma unroll
-    for (int i = 0; i < MxPart<TYPE, 32>::kWords / 4; ++i) {
-      const uint4 u = __ldg(p + i);
-      v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
-    }
-  } else {
-    typename Elem<TYPE>::T t[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t[i] = c0 + i < cols ? row[c0 + i] : Elem<TYPE>::put(0.f);
-    memcpy(v.w, t, sizeof(v.w));
-  }
-}
-
-// Codes and scale byte of a whole block.
-template <int TYPE>
-__device__ __forceinline__ uint32_t quantize_block(const MxPart<TYPE, 32>& v, uint4& q) {
-  float inv;
-  const uint32_t s = mx_scale(v.amax(), inv);
-  uint32_t w[4];
-  v.codes(inv, w);
-  q = make_uint4(w[0], w[1], w[2], w[3]);
-  return s;
-}
-
 // GGUF blocks of 32 values as source (quant.rs:135-190): Q4_0 holds elements
 // 0..15 in the low nibbles and 16..31 in the high ones, offset by 8.
 __device__ __forceinline__ void load_gguf_block(const uint8_t* blk, bool q4, MxPart<kF32, 32>& part) {

@@ -58,6 +58,9 @@ using tc::wait_bar;
 
 constexpr int kStages = 5;
 constexpr int kThreads = 384;
+constexpr int kFewTokens = 16, kFewWarps = 10;                   // tokens that a CTA quantises itself, and its warps for it
+constexpr int kFewChunkBytes = 1024 + kFewTokens * kMxChunk * 16;  // their scales and codes per K chunk
+constexpr int kFewCols = 8192;
 constexpr int kExPitch = 33;                          // f32 per row of the GeGLU exchange
 constexpr int kExBytes = 2 * kMxRows * kExPitch * 4;  // two groups' 128 rows x 32 tokens
 
@@ -87,6 +90,9 @@ struct Params {
   long long ldo;
   uint8_t* act;            // gated: MXFP4 [token row][n_out]
   int* err;
+  const void* raw;         // unquantised tokens [n_tokens][ldx], cols columns (QT >= 0)
+  long long ldx;
+  int cols, raw_vec;
   // Nothing but the tokens (and, for the GeGLU's result, earlier readers of
   // act) comes from the kernel right before this one, and that kernel let this
   // one start only after its own predecessors had completed: then the unit
@@ -95,7 +101,7 @@ struct Params {
 };
 
 struct __align__(8) Bars {
-  uint64_t full[kStages], empty[kStages], peer_full[kStages], acc_full[2], acc_empty[2], drain;
+  uint64_t full[kStages], empty[kStages], peer_full[kStages], acc_full[2], acc_empty[2], drain, tokens;
   uint32_t tmem_base;
   int abort;
   int first[kMaxExperts + 1];  // token tiles of earlier experts
@@ -320,11 +326,11 @@ struct Issue {
 };
 
 // A chunk of n blocks (even): its scales to tensor memory, then n / 2 MMAs.
-// wa: descriptor low word of the stage; sf: the stage's scale columns.
+// wa, xs: descriptor low words of the weights' chunk and of the tokens' scales,
+// which their codes follow; sf: the stage's scale columns.
 template <bool kPair, int n>
-__device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t sf, bool add) {
+__device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t xs, uint32_t sf, bool add) {
   constexpr int kGroups = (n + 3) / 4, kTiles = Shape<kPair>::kTokenTiles;
-  const uint32_t xs = wa + (kMxChunkBytes >> 4);
   // one tile's scales are directly followed by its codes (mx4.cuh)
   const uint32_t xa = xs + (kPair ? Shape<kPair>::kTokenScales >> 4 : 32 * kGroups);
 #pragma unroll
@@ -341,10 +347,13 @@ __device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t 
 
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
 
-template <int MODE, bool kPair>
+// QT >= 0: the tokens come unquantised, as QT, at most kFewTokens of them in one
+// matrix: every CTA quantises them all into its own shared memory, where they
+// stay, and only the weights pass through the ring.  One launch instead of two.
+template <int MODE, bool kPair, int QT = -1>
 __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   using S = Shape<kPair>;
-  constexpr int kStageBytes = S::kStageBytes;
+  constexpr int kStageBytes = QT >= 0 ? kMxChunkBytes : S::kStageBytes;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Bars* B = reinterpret_cast<Bars*>(smem_raw);
   uint8_t* ring = smem_raw + kBarBytes;
@@ -354,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&B->full[i], 2);
+      mbar_init(&B->full[i], QT >= 0 ? 1 : 2);
       mbar_init(&B->empty[i], 1);
       mbar_init(&B->peer_full[i], 1);
     }
@@ -363,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       mbar_init(&B->acc_empty[i], kPair ? 16 : 8);
     }
     mbar_init(&B->drain, 1);
+    mbar_init(&B->tokens, kFewWarps);
     B->abort = 0;
     fence_barrier_init();
   }
@@ -417,7 +427,29 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   // computed, and whole chunks have constant sizes.
   const int n_full = P.nb / kMxChunk, n_tail = P.nb % kMxChunk;
   const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(&B->full[0]), empty0 = smem_u32(&B->empty[0]);
-  if (warp == 0 || warp == 2) {
+  if (QT >= 0 && warp >= 2) {
+    // the tokens: a thread per (token, block); then to their other roles
+    constexpr int kType = QT >= 0 ? QT : kF32;
+    uint8_t* few = ring + kStages * kStageBytes;
+    for (int i = threadIdx.x - 64; i < P.n_tokens * P.nb; i += 32 * kFewWarps) {
+      const int t = i / P.nb, b = i % P.nb, c = b / kMxChunk, bl = b % kMxChunk;
+      MxPart<kType, 32> v;
+      if (b * 32 < P.cols)
+        load_block<kType>(static_cast<const typename Elem<kType>::T*>(P.raw) + t * P.ldx, b, P.cols, P.raw_vec, v);
+      else
+        v.zero();
+      uint4 q;
+      const uint32_t s = quantize_block(v, q);
+      const int n = min(kMxChunk, P.nb - c * kMxChunk);
+      uint8_t* chunk = few + c * kFewChunkBytes;
+      *reinterpret_cast<uint4*>(chunk + mx_scale_bytes(n) + (t >> 3) * (n * 128) + bl * 128 + (t & 7) * 16) = q;
+      chunk[(bl >> 2) * 512 + t * 16 + (bl & 3)] = (uint8_t)s;
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B->tokens);
+  }
+  if (warp == 0 || (QT < 0 && warp == 2)) {
     if (elect_one()) {
       // Warp 0 copies the weights, warp 2 the tokens: one thread for both was
       // what bounded the pairs' chunks (up to five copies each).
@@ -486,6 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       int s = 0, a = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
+      if (QT >= 0) ok = wait_at(smem_u32(&B->tokens), 0, B, P.err);
       Units<kPair> U;
       for (U.start(P, B); U.u < n_units && ok; U.u += step) {
         U.locate(P, B);
@@ -494,11 +527,14 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
                       U.row0 % kMxRows + N > kMxRows};
         if (!(ok = wait_at(smem_u32(&B->acc_empty[a]), aph ^ 1, B, P.err))) break;
         fence_after();
+        uint32_t few = desc_lo(ring0 + kStages * kStageBytes);
         auto chunk = [&](auto issue, bool add) {
           if (!wait_at(full0 + 8 * s, ph, B, P.err)) return false;
           if (kPair && !wait_at(smem_u32(&B->peer_full[s]), ph, B, P.err)) return false;
           fence_after();
-          issue(I, desc_lo(ring0 + s * kStageBytes), tmem + S::kSf0 + s * S::kSfCols, add);
+          const uint32_t wa = desc_lo(ring0 + s * kStageBytes);
+          issue(I, wa, QT >= 0 ? few : wa + (kMxChunkBytes >> 4), tmem + S::kSf0 + s * S::kSfCols, add);
+          few += kFewChunkBytes >> 4;
           commit<kPair>(&B->empty[s]);
           if (++s == kStages) {
             s = 0;
@@ -633,11 +669,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   }
 }
 
-template <int MODE, bool kPair>
+template <int MODE, bool kPair, int QT = -1>
 cudaError_t launch(const Params& P, long long units, cudaStream_t s) {
   static SmemOptIn cache;
-  const size_t smem = kBarBytes + kStages * Shape<kPair>::kStageBytes + (MODE == kModeGated ? kExBytes : 0);
-  const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE, kPair>, smem, cache);
+  const size_t smem = QT >= 0 ? kBarBytes + kStages * kMxChunkBytes + (P.nb + kMxChunk - 1) / kMxChunk * kFewChunkBytes
+                              : kBarBytes + kStages * Shape<kPair>::kStageBytes + (MODE == kModeGated ? kExBytes : 0);
+  const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE, kPair, QT>, smem, cache);
   if (st != cudaSuccess) return st;
   const int ctas = kPair ? 2 : 1;
   const int grid = ctas * (int)std::max<long long>(1, std::min<long long>(units, tc_num_sms() / ctas));
@@ -653,7 +690,7 @@ cudaError_t launch(const Params& P, long long units, cudaStream_t s) {
   attr[1].val.clusterDim = {2, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = kPair ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<MODE, kPair>, P);
+  return cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<MODE, kPair, QT>, P);
 }
 
 template <bool kPair>
@@ -697,6 +734,31 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   if (tokens >= 192ll * E && 2 * tiles >= 9ll * tc_num_sms() && cols >= 1024)
     return mx::launch_mode<true>(mode, P, (tokens / 192 + E) * ((P.w_tiles + 1) / 2), s);
   return mx::launch_mode<false>(mode, P, (tokens / 128 + std::min<long long>(E, tokens)) * P.w_tiles, s);
+}
+
+bool mx4_few_tokens(int tokens, int cols) { return tokens <= mx::kFewTokens && cols <= mx::kFewCols; }
+
+cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long ldx, int n_tokens, int rows, int cols,
+                           void* out, long long ldo, int* err, cudaStream_t s) {
+  mx::Params P{};
+  P.w = w;
+  P.E = 1;
+  P.n_tokens = n_tokens;
+  P.w_tiles = (rows + kMxRows - 1) / kMxRows;
+  P.nb = mx_blocks(cols);
+  P.n_out = rows;
+  P.out = out;
+  P.ldo = ldo;
+  P.err = err;
+  P.raw = x;
+  P.ldx = ldx;
+  P.cols = cols;
+  P.raw_vec = ((uintptr_t)x & 15) == 0 && (size_t)ldx * elem_bytes(type) % 16 == 0;
+  switch (type) {
+    case kF32: return mx::launch<mx::kModeF32, false, kF32>(P, P.w_tiles, s);
+    case kF16: return mx::launch<mx::kModeF16, false, kF16>(P, P.w_tiles, s);
+    default: return mx::launch<mx::kModeBF16, false, kBF16>(P, P.w_tiles, s);
+  }
 }
 
 }  // namespace mrml

@@ -280,6 +280,12 @@ int mrml_moe_mx4_linear(int type, const void* x, int64_t ldx, const uint8_t* w, 
   const size_t mm = mrml_moe_mx4_matmul_workspace_bytes(T, N, K);
   uint8_t* xq = static_cast<uint8_t*>(workspace) + mm;
   if (!aligned16(w) || !elem_aligned(x, type) || !elem_aligned(out, type)) return MRML_ERR_INVALID_ARGUMENT;
+  if (mrml::mx4_few_tokens(T, K)) {
+    MRML_TRY(mrml::check_device());
+    const cudaStream_t s = (cudaStream_t)stream;
+    MRML_LAUNCH(mrml::launch_mx4_few(type, w, x, ldx, T, N, K, out, ldo, static_cast<int*>(workspace), s));
+    return MRML_OK;
+  }
   MRML_TRY(mrml_moe_mx4_quantize(type, x, ldx, 0, xq, T, K, 1, 0, stream));
   return matmul(type, xq, w, out, ldo, T, N, K, workspace, mm, true, stream);
 }

@@ -238,6 +238,9 @@ PRODUCTS = [
     # chunks of every length
     (192, 128, 64), (193, 129, 96), (384, 640, 320), (400, 257, 448), (575, 300, 1000), (1000, 130, 704), (2000, 900, 512),
     (4000, 3330, 1056), (9001, 1500, 1100), (12300, 1000, 1216), (100000, 130, 1024),
+    # a few tokens, quantised by the product itself, up to and past its longest sum
+    (2, 300, 33), (7, 129, 448), (8, 64, 704), (9, 1000, 96), (15, 260, 1000), (16, 4224, 2816), (3, 130, 8192),
+    (2, 64, 8200), (1, 20000, 64),
 ]
 
 
@@ -257,6 +260,12 @@ def test_product(cuda, moe, M, N, K, dtype):
     moe.mx4_linear(x, qw, out, M, N, K, ws)
     assert moe.device_status(ws)[0] == 0
     check_product(out, a, b, dtype)
+    # unaligned rows of x give the same
+    _, xs = strided(M, K, dtype, cuda, 5, 1)
+    xs.copy_(x)
+    again = torch.full((M, N), 7.0, dtype=dtype, device=cuda)
+    moe.mx4_linear(xs, qw, again, M, N, K, ws)
+    assert torch.equal(again, out)
     out.fill_(7.0)
     assert (buf == 7.0).all(), "written outside the output"
 
