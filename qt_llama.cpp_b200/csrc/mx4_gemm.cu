@@ -90,6 +90,10 @@ struct Params {
   long long ldo;
   uint8_t* act;            // gated: MXFP4 [token row][n_out]
   int* err;
+  // A few (token, slot) pairs instead of sorted rows: pair p is alone in token
+  // tile p, with the weights of expert ids[p] (left out if there is none).
+  const int32_t* ids;
+  int pairs, K;
   const void* raw;         // unquantised tokens [n_tokens][ldx], cols columns (QT >= 0)
   long long ldx;
   int cols, raw_vec;
@@ -277,7 +281,7 @@ template <bool kPair>
 struct Units {
   static constexpr int kTokens = Shape<kPair>::kTokens;
   int u, e, w_units, first, next;  // unit; expert, its first unit and the next expert's
-  int wt, row0, n;
+  int wt, row0, n, col;            // col: first token's column in the accumulator
   size_t w_tile;
 
   __device__ __forceinline__ void start(const Params& P, const Bars* B) {
@@ -288,7 +292,16 @@ struct Units {
     next = P.offsets ? B->first[1] * w_units : 0x7fffffff;
   }
   __device__ __forceinline__ void locate(const Params& P, const Bars* B) {
-    if (P.offsets) {
+    col = 0;
+    if (P.ids) {
+      const unsigned j = (unsigned)u / (unsigned)P.w_tiles;
+      const int p = B->row0[j];
+      wt = (int)(u - j * P.w_tiles);
+      e = B->count[j];
+      row0 = p * kMxRows;
+      n = 1;
+      if (P.raw) col = p / P.K;  // all tokens are multiplied, one of them is meant
+    } else if (P.offsets) {
       while (u >= next) {  // u is below the last expert's end
         ++e;
         first = next;
@@ -357,7 +370,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Bars* B = reinterpret_cast<Bars*>(smem_raw);
   uint8_t* ring = smem_raw + kBarBytes;
-  float* ex = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // GeGLU exchange
+  float* ex = reinterpret_cast<float*>(ring + kStages * kStageBytes +  // GeGLU exchange
+                                       (QT >= 0 ? (P.nb + kMxChunk - 1) / kMxChunk * kFewChunkBytes : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? (int)(blockIdx.x & 1) : 0;  // in the cluster of two
 
@@ -387,6 +401,18 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   }
   if (!P.early) pdl_wait();
   pdl_trigger();
+  if (P.ids && warp == 3) {  // the pairs that have an expert
+    const int id = lane < P.pairs ? P.ids[lane] : -1;
+    const bool has = (unsigned)id < (unsigned)P.E;
+    const unsigned all = __ballot_sync(0xffffffffu, has);
+    if (has) {
+      const int j = __popc(all & ((1u << lane) - 1));
+      B->row0[j] = lane;
+      B->count[j] = id;
+    }
+    if (lane == 0) B->first[0] = __popc(all);
+    if (id >= P.E && blockIdx.x == 0) set_error(P.err, kDevBadExpert);
+  }
   if (P.offsets && warp == 3) {  // token tiles before each expert
     constexpr int kPer = kMaxExperts / 32;
     int c[kPer], s = 0;
@@ -417,7 +443,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   else __syncthreads();
   fence_after();
   const uint32_t tmem = B->tmem_base;
-  const int n_units = (P.offsets ? B->first[P.E] : (P.n_tokens + S::kTokens - 1) / S::kTokens) *
+  const int n_units = (P.ids       ? B->first[0]
+                       : P.offsets ? B->first[P.E]
+                                   : (P.n_tokens + S::kTokens - 1) / S::kTokens) *
                       (kPair ? (P.w_tiles + 1) / 2 : P.w_tiles);
   const int step = (int)gridDim.x / (kPair ? 2 : 1);
   const size_t tile_bytes = mx_tile_bytes(P.nb);
@@ -522,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       Units<kPair> U;
       for (U.start(P, B); U.u < n_units && ok; U.u += step) {
         U.locate(P, B);
-        const int N = (U.n + 15) & ~15, M = kPair ? 2 * kMxRows : kMxRows;
+        const int N = QT >= 0 ? kFewTokens : (U.n + 15) & ~15, M = kPair ? 2 * kMxRows : kMxRows;
         const Issue I{tmem + a * S::kTokens, idesc(M, N, 0), idesc(M, N, 2), (uint32_t)(U.row0 % kMxRows / 32),
                       U.row0 % kMxRows + N > kMxRows};
         if (!(ok = wait_at(smem_u32(&B->acc_empty[a]), aph ^ 1, B, P.err))) break;
@@ -590,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       else ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + a * S::kTokens;
+      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + a * S::kTokens + U.col;
       uint32_t r[32];
       if constexpr (MODE == kModeGated) {
         // 32 tokens at a time: all rows to shared memory (rows 0..63 gate,
@@ -672,8 +700,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
 template <int MODE, bool kPair, int QT = -1>
 cudaError_t launch(const Params& P, long long units, cudaStream_t s) {
   static SmemOptIn cache;
-  const size_t smem = QT >= 0 ? kBarBytes + kStages * kMxChunkBytes + (P.nb + kMxChunk - 1) / kMxChunk * kFewChunkBytes
-                              : kBarBytes + kStages * Shape<kPair>::kStageBytes + (MODE == kModeGated ? kExBytes : 0);
+  const size_t smem = kBarBytes + (MODE == kModeGated ? kExBytes : 0) +
+                      (QT >= 0 ? kStages * kMxChunkBytes + (P.nb + kMxChunk - 1) / kMxChunk * kFewChunkBytes
+                               : kStages * Shape<kPair>::kStageBytes);
   const cudaError_t st = ensure_smem(mx4_gemm_kernel<MODE, kPair, QT>, smem, cache);
   if (st != cudaSuccess) return st;
   const int ctas = kPair ? 2 : 1;
@@ -736,7 +765,12 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   return mx::launch_mode<false>(mode, P, (tokens / 128 + std::min<long long>(E, tokens)) * P.w_tiles, s);
 }
 
-bool mx4_few_tokens(int tokens, int cols) { return tokens <= mx::kFewTokens && cols <= mx::kFewCols; }
+// About one block per quantising thread: 4 tokens of 2816 take 6.0 us in one
+// launch and 5.8 in two, 1 token 5.0 and 5.9, 16 tokens 7.9 and 5.9 (4224
+// outputs); 16 tokens of 704 4.6 and 4.6 (2816 outputs).
+bool mx4_few_tokens(int tokens, int cols) {
+  return tokens <= mx::kFewTokens && cols <= mx::kFewCols && (long long)tokens * mx_blocks(cols) <= 384;
+}
 
 cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long ldx, int n_tokens, int rows, int cols,
                            void* out, long long ldo, int* err, cudaStream_t s) {
@@ -759,6 +793,57 @@ cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long 
     case kF16: return mx::launch<mx::kModeF16, false, kF16>(P, P.w_tiles, s);
     default: return mx::launch<mx::kModeBF16, false, kBF16>(P, P.w_tiles, s);
   }
+}
+
+// A few pairs of tokens that a CTA can quantise itself, and no more of them
+// than experts: then hardly two share one, and sorting them saves nothing.
+bool mx4_few_pairs(int T, int K, int E, int H) {
+  return (long long)T * K <= std::min(32, E) && mx4_few_tokens(T, H);
+}
+
+cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids, int T,
+                                   int K, int E, int H, int I, uint8_t* act, int* err, cudaStream_t s) {
+  mx::Params P{};
+  P.w = w;
+  P.E = E;
+  P.n_tokens = T;
+  P.w_tiles = (2 * I + kMxRows - 1) / kMxRows;
+  P.nb = mx_blocks(H);
+  P.n_out = I;
+  P.act = act;
+  P.err = err;
+  P.ids = ids;
+  P.pairs = T * K;
+  P.K = K;
+  P.raw = x;
+  P.ldx = ldx;
+  P.cols = H;
+  P.raw_vec = ((uintptr_t)x & 15) == 0 && (size_t)ldx * elem_bytes(type) % 16 == 0;
+  const long long units = (long long)T * K * P.w_tiles;
+  switch (type) {
+    case kF32: return mx::launch<mx::kModeGated, false, kF32>(P, units, s);
+    case kF16: return mx::launch<mx::kModeGated, false, kF16>(P, units, s);
+    default: return mx::launch<mx::kModeGated, false, kBF16>(P, units, s);
+  }
+}
+
+cudaError_t launch_mx4_few_down(const uint8_t* w, const uint8_t* act, const int32_t* ids, int T, int K, int E, int H,
+                                int I, float* y, int* err, cudaStream_t s) {
+  mx::Params P{};
+  P.w = w;
+  P.x = act;
+  P.E = E;
+  P.w_tiles = (H + kMxRows - 1) / kMxRows;
+  P.nb = mx_blocks(I);
+  P.n_out = H;
+  P.out = y;
+  P.ldo = H;
+  P.err = err;
+  P.ids = ids;
+  P.pairs = T * K;
+  P.K = K;
+  P.early = 1;  // ids and weights are older than the launch before
+  return mx::launch<mx::kModeF32, false>(P, (long long)T * K * P.w_tiles, s);
 }
 
 }  // namespace mrml

@@ -400,6 +400,10 @@ LAYERS = [
     (2048, 2, 16, 256, 128, 0.0, None),
     (700, 4, 8, 416, 352, 0.1, None), (1500, 2, 5, 320, 96, 0.0, 4), (900, 8, 16, 264, 200, 0.2, None),
     (4100, 4, 8, 1088, 700, 0.1, None), (3000, 8, 7, 1040, 333, 0.0, None),
+    # few enough pairs to go unsorted: dropped slots, all dropped, slots that share an expert, the largest
+    (1, 8, 128, 2816, 704, 0.0, None), (1, 8, 9, 96, 40, 0.4, None), (2, 4, 8, 320, 100, 1.0, None),
+    (3, 4, 16, 1001, 70, 0.0, 5), (4, 8, 32, 2816, 96, 0.1, None), (16, 2, 61, 704, 130, 0.2, None),
+    (1, 32, 64, 8192, 64, 0.0, None),
     # large batches, more than 8 slots
     (2048, 8, 16, 1024, 64, 0.0, None), (6000, 8, 9, 600, 96, 0.05, None), (1500, 12, 24, 1001, 40, 0.3, None),
 ]
@@ -449,12 +453,14 @@ def test_experts_strides_graph_and_bad_ids(cuda, moe):
     torch.cuda.synchronize()
     want, tol = experts_reference(c, T, K, E, H, I)
     assert ((out.double() - want).abs() <= tol).all()
-    # an id past the experts is left out and reported
-    c["ids"][5, 2] = E
-    out, ws = run_experts(moe, c, T, K, E, H, I)
-    assert moe.device_status(ws)[0] == -7
-    want, tol = experts_reference(c, T, K, E, H, I)
-    assert ((out.double() - want).abs() <= tol).all()
+    # an id past the experts is left out and reported, also among a few pairs
+    c["ids"][3, 2] = E
+    for rows in (T, 4):
+        d = dict(c, **{n: c[n][:rows].contiguous() for n in ("ids", "probs", "x")})
+        out, ws = run_experts(moe, d, rows, K, E, H, I)
+        assert moe.device_status(ws)[0] == -7
+        want, tol = experts_reference(d, rows, K, E, H, I)
+        assert ((out.double() - want).abs() <= tol).all()
 
 
 def test_experts_keep_non_finite_tokens_apart(cuda, moe):
