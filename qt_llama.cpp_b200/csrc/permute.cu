@@ -20,9 +20,9 @@ namespace {
 // Counting sort, stable by construction: a warp owns consecutive pairs, ranks
 // those of one expert with a warp match, and starts from the counts of the
 // warps (and chunks) before it.  No atomic decides an order.  Bound by latency:
-// 64 pairs 3.4 us, 512 pairs 6.9 us in one CTA of few warps; 65536 pairs in two
-// launches 3.4 + 9.1 us, whose chunks each sum all chunks' counts instead of
-// waiting for a scan in between.
+// 64 pairs 2.8 us, 512 pairs 4.1 us in one CTA; 65536 pairs in two launches 7.9
+// us, whose chunks each sum all chunks' counts instead of waiting for a scan in
+// between.
 struct SortArgs {
   const int32_t* ids;
   int32_t *offsets, *counts, *pos, *pair;
@@ -358,9 +358,10 @@ bool rows_aligned(const void* p, long long ld, size_t s) { return ((uintptr_t)p 
 
 }  // namespace
 
-// Pairs up to which one CTA sorts (ITEMS pairs per thread), and the chunk of
-// the larger sorts, whose two launches read the ids twice.
-constexpr int kSortOne = 4096;
+// Pairs up to which one CTA sorts, and the chunk of the larger sorts, whose two
+// launches read the ids twice: 4096 pairs take 11.3 us in one CTA and 6.4 in
+// chunks, 1024 pairs 5.4 in one.
+constexpr int kSortOne = 1024;
 
 int sort_chunk(long long n_pairs) { return n_pairs <= (1 << 19) ? 1024 : 8192; }
 
@@ -374,9 +375,10 @@ cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, i
                         int n_pairs, int align, int n_rows, int32_t* chunk_cnt, int* err, cudaStream_t s) {
   SortArgs a{ids, offsets, counts, pos, pair, chunk_cnt, err, n_pairs, E, align, n_rows, 0};
   const bool one = n_pairs <= kSortOne;
-  // one CTA: few warps, whose counts are scanned one after another
-  const int items = one ? (n_pairs <= 256 ? 1 : 4) : sort_chunk(n_pairs) / 1024;
-  const int threads = one ? (n_pairs <= 1024 ? 256 : 1024) : 1024;
+  // one CTA: no more warps than pairs for them, as their counts are scanned one
+  // after another (512 pairs: 4.1 us in 512 threads, 5.3 in 256 with four each)
+  const int items = one ? 1 : sort_chunk(n_pairs) / 1024;
+  const int threads = one ? std::max(256, (n_pairs + 255) / 256 * 256) : 1024;
   a.chunk = items * threads;
   const int grid = std::max(1, (n_pairs + a.chunk - 1) / a.chunk);
   const size_t smem = (size_t)(threads / 32 * E + 3 * E + 1) * 4;
@@ -386,7 +388,6 @@ cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, i
   }
   switch (items) {
     case 1: return launch_pdl(sort_place_kernel<1>, dim3(grid), dim3(threads), smem, s, a);
-    case 4: return launch_pdl(sort_place_kernel<4>, dim3(grid), dim3(threads), smem, s, a);
     default: return launch_pdl(sort_place_kernel<8>, dim3(grid), dim3(threads), smem, s, a);
   }
 }
