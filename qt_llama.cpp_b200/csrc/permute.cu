@@ -20,7 +20,7 @@ namespace {
 // Counting sort, stable by construction: a warp owns consecutive pairs, ranks
 // those of one expert with a warp match, and starts from the counts of the
 // warps (and chunks) before it.  No atomic decides an order.  Bound by latency:
-// 64 pairs 2.8 us, 512 pairs 4.1 us in one CTA; 65536 pairs in two launches 7.9
+// 64 pairs 2.8 us, 512 pairs 4.1 us in one CTA; 65536 pairs in two launches 7.1
 // us, whose chunks each sum all chunks' counts instead of waiting for a scan in
 // between.
 struct SortArgs {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
       int all = 0, mine = 0;
 #pragma unroll 8
       for (int c = threadIdx.x / E; c < chunks; c += step) {
-        const int n = __ldg(a.chunk_cnt + (size_t)c * E + x);
+        const int n = a.chunk_cnt[(size_t)c * E + x];
         all += n;
         if (c < (int)blockIdx.x) mine += n;
       }
@@ -359,11 +359,13 @@ bool rows_aligned(const void* p, long long ld, size_t s) { return ((uintptr_t)p 
 }  // namespace
 
 // Pairs up to which one CTA sorts, and the chunk of the larger sorts, whose two
-// launches read the ids twice: 4096 pairs take 11.3 us in one CTA and 6.4 in
-// chunks, 1024 pairs 5.4 in one.
+// launches read the ids twice: 4096 pairs take 11.3 us in one CTA and 6.1 in
+// chunks, 1024 pairs 5.4 in one.  Every chunk reads all chunks' counts, so many
+// pairs take larger ones: chunks of 1024 and of 8192 pairs take 12.4 and 21.5 us
+// for 262144 pairs, 31 and 22 for 524288, 78 and 25 for 2^20.
 constexpr int kSortOne = 1024;
 
-int sort_chunk(long long n_pairs) { return n_pairs <= (1 << 19) ? 1024 : 8192; }
+int sort_chunk(long long n_pairs) { return n_pairs <= 3 << 17 ? 1024 : 8192; }
 
 size_t sort_chunk_ints(long long n_pairs, int E) {
   if (n_pairs <= kSortOne) return 0;

@@ -406,6 +406,7 @@ LAYERS = [
     (1, 32, 64, 8192, 64, 0.0, None),
     # large batches, more than 8 slots
     (2048, 8, 16, 1024, 64, 0.0, None), (6000, 8, 9, 600, 96, 0.05, None), (1500, 12, 24, 1001, 40, 0.3, None),
+    (3200, 8, 16, 1088, 96, 0.1, None), (2500, 12, 24, 1001, 40, 0.3, None),
 ]
 
 
