@@ -22,6 +22,8 @@ bool elem_aligned(const void* p, int type) { return ((uintptr_t)p & (mrml::elem_
 // The most (token, slot) pairs of a call: every chunk of a large sort sums the
 // counts of all chunks, which beyond this would take longer than the rest.
 constexpr long long kMaxPairs = 1ll << 26;
+// The widest row, and the most sorted rows: the kernels' column and row indices are ints.
+constexpr int kMaxCols = 1 << 24, kMaxRows = 0x7fffff00;
 
 // Rows of the sorted order, padding included; -1 when the arguments are
 // invalid.
@@ -36,7 +38,7 @@ long long rows_bound(int E, int K, int T, int align) {
 int check_tokens(int type, int H, int K, int T) {
   if (!is_float(type)) return MRML_ERR_UNSUPPORTED;
   if (H <= 0 || K <= 0 || T < 0) return MRML_ERR_INVALID_ARGUMENT;
-  if (K > kMaxTopK || (long long)T * K > kMaxPairs) return MRML_ERR_UNSUPPORTED;
+  if (H > kMaxCols || K > kMaxTopK || (long long)T * K > kMaxPairs) return MRML_ERR_UNSUPPORTED;
   // the gather takes a warp per 1024 values of a token
   if ((long long)T * ((H + 1023) / 1024) > 0x7fffffffll) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
@@ -51,7 +53,7 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 // 128 (dequantiser), 64 x 128 (both directions).
 int check_matrix(int rows, int cols, int matrices) {
   if (rows < 0 || cols <= 0 || matrices < 0) return MRML_ERR_INVALID_ARGUMENT;
-  if (matrices > 65535 || rows > 0x7fffff00 || cols > 0x7fffff00) return MRML_ERR_UNSUPPORTED;
+  if (matrices > 65535 || rows > kMaxRows || cols > kMaxRows) return MRML_ERR_UNSUPPORTED;
   if (((long long)rows + 127) / 16 * (((long long)cols + 127) / 128) > 0x7fffffffll) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
 }
@@ -106,7 +108,7 @@ ExpertsWs carve_experts(void* base, int H, int I, int E, int K, int T) {
 int check_product(int type, int M, int N, int K) {
   if (!is_float(type)) return MRML_ERR_UNSUPPORTED;
   if (M < 0 || N <= 0 || K <= 0) return MRML_ERR_INVALID_ARGUMENT;
-  if (M > 0x7fffff00 || N > 0x7fffff00 || K > (1 << 24)) return MRML_ERR_UNSUPPORTED;  // offsets in a tile fit an int
+  if (M > kMaxRows || N > kMaxRows || K > kMaxCols) return MRML_ERR_UNSUPPORTED;  // offsets in a tile fit an int
   if (((long long)M + 127) / 128 * (((long long)N + 127) / 128) > (1ll << 30)) return MRML_ERR_UNSUPPORTED;
   return MRML_OK;
 }
@@ -159,6 +161,7 @@ int mrml_moe_permute(int type, const void* x, int64_t ldx, const int32_t* pair, 
                      mrml_stream_t stream) {
   MRML_TRY(check_tokens(type, H, K, 0));
   if (n_rows < 0 || ldx < H) return MRML_ERR_INVALID_ARGUMENT;
+  if (n_rows > kMaxRows) return MRML_ERR_UNSUPPORTED;
   if (n_rows == 0) return MRML_OK;
   if (!x || !pair || !rows || !elem_aligned(x, type) || !elem_aligned(rows, type)) return MRML_ERR_INVALID_ARGUMENT;
   MRML_TRY(mrml::check_device());
@@ -189,6 +192,7 @@ int mrml_moe_unpermute_grad(int type, const void* dout, int64_t lddout, const vo
                             int n_rows, mrml_stream_t stream) {
   MRML_TRY(check_tokens(type, H, K, T));
   if (lddout < H || n_rows < 0) return MRML_ERR_INVALID_ARGUMENT;
+  if (n_rows > kMaxRows) return MRML_ERR_UNSUPPORTED;
   if (T == 0 || (!drows && !dprobs)) return MRML_OK;
   if (n_rows < T * K && drows) return MRML_ERR_INVALID_ARGUMENT;
   if (!dout || !pos || (drows && !pair) || (dprobs && !rows)) return MRML_ERR_INVALID_ARGUMENT;

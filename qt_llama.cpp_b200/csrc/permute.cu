@@ -365,12 +365,16 @@ bool rows_aligned(const void* p, long long ld, size_t s) { return ((uintptr_t)p 
 // for 262144 pairs, 31 and 22 for 524288, 78 and 25 for 2^20.
 constexpr int kSortOne = 1024;
 
-int sort_chunk(long long n_pairs) { return n_pairs <= 3 << 17 ? 1024 : 8192; }
+constexpr long long kSortSmallChunks = 3 << 17;
 
+int sort_chunk(long long n_pairs) { return n_pairs <= kSortSmallChunks ? 1024 : 8192; }
+
+// Never less than fewer pairs take, so that a workspace serves them too.
 size_t sort_chunk_ints(long long n_pairs, int E) {
   if (n_pairs <= kSortOne) return 0;
   const int c = sort_chunk(n_pairs);
-  return (size_t)((n_pairs + c - 1) / c) * E;
+  const long long chunks = (n_pairs + c - 1) / c;
+  return (size_t)(n_pairs > kSortSmallChunks ? std::max(chunks, kSortSmallChunks / 1024) : chunks) * E;
 }
 
 cudaError_t launch_sort(const int32_t* ids, int32_t* offsets, int32_t* counts, int32_t* pos, int32_t* pair, int E,

@@ -34,6 +34,27 @@ def test_sorted_rows_and_sizes(moe):
     assert lib.mrml_moe_mx4_experts_workspace_bytes(0, 704, 128, 8, 64) == 0
 
 
+def test_a_workspace_serves_fewer_tokens(moe):
+    lib = moe.load_library()
+    for K in (1, 2, 8, 64):
+        tokens = sorted({max(0, n // K + d) for n in (1, 32, 384, 512, 1024, 8192, 24576, 393216, 1 << 19, 1 << 22)
+                         for d in (-1, 0, 1, 2)})
+        for size in (lambda T: lib.mrml_moe_sort_workspace_bytes(256, K, T),
+                     lambda T: lib.mrml_moe_mx4_experts_workspace_bytes(32, 32, 16, K, T),
+                     lambda T: lib.mrml_moe_mx4_linear_workspace_bytes(T, 64, 96)):
+            sizes = [size(T) for T in tokens]
+            assert sizes == sorted(sizes)
+
+
+def test_sizes_past_the_index_types_are_refused(moe):
+    lib = moe.load_library()
+    top = 2**31 - 1
+    assert lib.mrml_moe_permute(0, P, top, P, P, top, 2, 4, None) == -2
+    assert lib.mrml_moe_permute(0, P, 64, P, P, 64, 2, top, None) == -2
+    assert lib.mrml_moe_unpermute(0, P, P, P, P, top, top, 2, 4, None) == -2
+    assert lib.mrml_moe_unpermute_grad(0, P, 64, P, P, P, P, P, P, 64, 2, 4, top, None) == -2
+
+
 def test_permutation_refusals(moe):
     lib = moe.load_library()
     sort = lib.mrml_moe_sort
