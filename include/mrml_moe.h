@@ -380,7 +380,8 @@ int mrml_moe_quantize_q4_0(const float *src, uint8_t *dst, size_t n, mrml_stream
  * slot order, and are rounded once; results do not vary between calls.
  * ld* are row strides in elements (at least H); the sorted rows are
  * contiguous.  Rows whose addresses and strides are multiples of 16 bytes
- * move in 16-byte vectors, others element by element. */
+ * move in 16-byte vectors, others element by element.  H <= 2^24, T*K <= 2^26.
+ * A workspace of T tokens serves fewer too, here and below. */
 
 /* Rows of the sorted order, an upper bound with each expert's rows padded to
  * a multiple of `align` (1..128): T*K + min(E, T*K) * (align - 1); negative
