@@ -208,10 +208,9 @@ cudaError_t launch_permute(int type, const void* x, long long ldx, const int32_t
 cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, const float* probs, void* out,
                              long long ldo, int H, int K, int T, cudaStream_t s);
 // The same from the expert layer's down products (f32 rows), with the weights
-// times scale[ids] (scale may be null).  pos null: pair p's row is 128 p if
-// ids[p] is in [0, E).
+// times scale[ids] (scale may be null).
 cudaError_t launch_combine_rows(int type, const float* rows, const int32_t* pos, const float* probs,
-                                const int32_t* ids, int E, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
                                 cudaStream_t s);
 cudaError_t launch_unpermute_grad(int type, const void* dout, long long ldd, const void* rows, const int32_t* pos,
                                   const int32_t* pair, const float* probs, void* drows, float* dprobs, int H, int K,
@@ -246,12 +245,13 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
 bool mx4_few_tokens(int tokens, int cols);
 cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long ldx, int n_tokens, int rows, int cols,
                            void* out, long long ldo, int* err, cudaStream_t s);
-// The expert layer's two products for a few (token, slot) pairs that are not
-// sorted (where mx4_few_pairs says so): pair p alone in token tile p, its row of
-// y at 128 p.
-bool mx4_few_pairs(int T, int K, int E, int H);
-cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids, int T,
-                                   int K, int E, int H, int I, uint8_t* act, int* err, cudaStream_t s);
+// The expert layer's two products for a few (token, slot) pairs (where
+// mx4_few_pairs says so), which their CTAs sort themselves: an expert's pairs
+// share a tile of rows, pos [T][K] (written by the first) is each pair's or -1.
+bool mx4_few_pairs(int T, int K, int H);
+cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids,
+                                   int32_t* pos, int T, int K, int E, int H, int I, uint8_t* act, int* err,
+                                   cudaStream_t s);
 cudaError_t launch_mx4_few_down(const uint8_t* w, const uint8_t* act, const int32_t* ids, int T, int K, int E, int H,
                                 int I, float* y, int* err, cudaStream_t s);
 int gate_up_tok_chunk(int wtype, int H);

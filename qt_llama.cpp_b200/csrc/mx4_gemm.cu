@@ -29,10 +29,11 @@
 // 192 x 256, and the first CTA's warp 1 issues for both.  The second CTA's
 // warp 1 passes on that its stage has landed.
 //
-// A few tokens come unquantised: every CTA quantises them into its own shared
-// memory, and in the expert layer each (token, slot) pair is a unit column of
-// its own instead of a place in sorted rows.  There is nothing to share, and a
-// launch costs more than the repeated work.
+// A few tokens come unquantised: every CTA quantises them all into its own
+// shared memory and, in the expert layer, sorts their (token, slot) pairs by
+// itself: launches for it cost more than the repeated work.  The gate and up
+// product multiplies all of them by each expert that has a pair (N = 16 is the
+// least that the tensor cores take) and keeps the pairs' columns.
 //
 // Measured (weights of a 128-expert layer, H = 2816, I = 704): 64 tokens' gate
 // and up product 40 us for 270 MB of weights and activations, 6.7 TB/s, the
@@ -66,6 +67,7 @@ constexpr int kThreads = 384;
 constexpr int kFewTokens = 16, kFewWarps = 10;                   // tokens that a CTA quantises itself, and its warps for it
 constexpr int kFewChunkBytes = 1024 + kFewTokens * kMxChunk * 16;  // their scales and codes per K chunk
 constexpr int kFewCols = 8192;
+constexpr int kFewPairs = 128;  // (token, slot) pairs that a CTA sorts itself: one expert's fit a tile
 constexpr int kExPitch = 33;                          // f32 per row of the GeGLU exchange
 constexpr int kExBytes = 2 * kMxRows * kExPitch * 4;  // two groups' 128 rows x 32 tokens
 
@@ -95,9 +97,10 @@ struct Params {
   long long ldo;
   uint8_t* act;            // gated: MXFP4 [token row][n_out]
   int* err;
-  // A few (token, slot) pairs instead of sorted rows: pair p is alone in token
-  // tile p, with the weights of expert ids[p] (left out if there is none).
+  // A few (token, slot) pairs instead of sorted rows: every CTA sorts them
+  // itself, the experts in the order of their first pairs, one tile each.
   const int32_t* ids;
+  int32_t* pos;            // [pairs] each pair's row or -1, written by one CTA; or null
   int pairs, K;
   const void* raw;         // unquantised tokens [n_tokens][ldx], cols columns (QT >= 0)
   long long ldx;
@@ -115,7 +118,12 @@ struct __align__(8) Bars {
   int abort;
   int first[kMaxExperts + 1];  // token tiles of earlier experts
   int row0[kMaxExperts], count[kMaxExperts];  // each expert's first row and rows
+  // of a few pairs: experts that have some; each one's id; pairs' tokens,
+  // expert by expert, and (row0) where an expert's start among them
+  int experts;
+  uint8_t expert[kFewPairs], token[kFewPairs];
 };
+static_assert(kMaxExperts <= 256 && kFewTokens <= 256, "expert and token numbers are kept in bytes");
 constexpr int kBarBytes = 4096;
 static_assert(sizeof(Bars) <= kBarBytes, "the barrier block must fit its part of shared memory");
 
@@ -286,7 +294,7 @@ template <bool kPair>
 struct Units {
   static constexpr int kTokens = Shape<kPair>::kTokens;
   int u, e, w_units, first, next;  // unit; expert, its first unit and the next expert's
-  int wt, row0, n, col;            // col: first token's column in the accumulator
+  int wt, row0, n, list;           // list: the first pair's place in Bars::token
   size_t w_tile;
 
   __device__ __forceinline__ void start(const Params& P, const Bars* B) {
@@ -297,15 +305,13 @@ struct Units {
     next = P.offsets ? B->first[1] * w_units : 0x7fffffff;
   }
   __device__ __forceinline__ void locate(const Params& P, const Bars* B) {
-    col = 0;
     if (P.ids) {
       const unsigned j = (unsigned)u / (unsigned)P.w_tiles;
-      const int p = B->row0[j];
       wt = (int)(u - j * P.w_tiles);
-      e = B->count[j];
-      row0 = p * kMxRows;
-      n = 1;
-      if (P.raw) col = p / P.K;  // all tokens are multiplied, one of them is meant
+      e = B->expert[j];
+      row0 = (int)j * kMxRows;
+      n = B->count[j];
+      list = B->row0[j];
     } else if (P.offsets) {
       while (u >= next) {  // u is below the last expert's end
         ++e;
@@ -363,6 +369,99 @@ __device__ __forceinline__ void chunk_mma(const Issue& I, uint32_t wa, uint32_t 
                     sf + (j >> 1) * 4, sf + 8 + 4 * kTiles * (j >> 1) + (kPair ? I.shift : 0), add || j > 0);
 }
 
+// A few pairs sorted by one warp: groups of 32 in turn, the experts numbered as
+// they appear (Bars::first holds the number, or -1), the pairs ranked within
+// theirs by a warp match.
+__device__ __forceinline__ void sort_few(const Params& P, Bars* B, int lane) {
+  constexpr int kGroups = kFewPairs / 32;
+  const unsigned below = (1u << lane) - 1;
+  if (P.pairs <= 32) {  // one group: no counts to carry over, 0.6 us less in a one-token layer
+    int id = lane < P.pairs ? P.ids[lane] : -1;
+    if (id >= P.E) {
+      if (blockIdx.x == 0) set_error(P.err, kDevBadExpert);
+      id = -1;
+    }
+    const bool has = id >= 0;
+    const unsigned same = __match_any_sync(0xffffffffu, has ? id : -1);
+    const int n = __popc(same), leader = __ffs(same) - 1, rank = __popc(same & below);
+    const bool lead = has && rank == 0;
+    const unsigned leads = __ballot_sync(0xffffffffu, lead);
+    const int j = __popc(leads & ((1u << leader) - 1));
+    int start = lead ? n : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, start, o);
+      if (lane >= o) start += y;
+    }
+    start = __shfl_sync(0xffffffffu, start - n, leader);
+    if (lead) {
+      B->expert[j] = (uint8_t)id;
+      B->count[j] = n;
+      B->row0[j] = start;
+    }
+    if (has) B->token[start + rank] = (uint8_t)(lane / P.K);
+    if (lane == 0) B->experts = __popc(leads);
+    if (P.pos && blockIdx.x == 0 && lane < P.pairs) P.pos[lane] = has ? j * kMxRows + rank : -1;
+    return;
+  }
+  for (int e = lane; e < P.E; e += 32) B->first[e] = -1;
+  for (int j = lane; j < kFewPairs; j += 32) B->count[j] = 0;
+  int id[kGroups], j[kGroups], rank[kGroups], experts = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) id[g] = 32 * g + lane < P.pairs ? P.ids[32 * g + lane] : -1;
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    if (32 * g >= P.pairs) break;
+    if (id[g] >= P.E) {
+      if (blockIdx.x == 0) set_error(P.err, kDevBadExpert);
+      id[g] = -1;
+    }
+    const bool has = id[g] >= 0;
+    if (!has) id[g] = -1;
+    const unsigned same = __match_any_sync(0xffffffffu, id[g]);
+    const bool lead = has && (same & below) == 0, fresh = lead && B->first[id[g]] < 0;
+    const unsigned all = __ballot_sync(0xffffffffu, fresh);
+    if (fresh) {
+      const int n = experts + __popc(all & below);
+      B->first[id[g]] = n;
+      B->expert[n] = (uint8_t)id[g];
+    }
+    experts += __popc(all);
+    __syncwarp();
+    if (has) {
+      j[g] = B->first[id[g]];
+      rank[g] = B->count[j[g]] + __popc(same & below);
+    }
+    __syncwarp();
+    if (lead) B->count[j[g]] += __popc(same);
+    __syncwarp();
+  }
+  if (lane == 0) B->experts = experts;
+  int c[kGroups], s = 0;  // where each expert's pairs start: kGroups experts per lane
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    c[i] = s;
+    s += B->count[lane * kGroups + i];
+  }
+  int up = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += y;
+  }
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) B->row0[lane * kGroups + i] = up - s + c[i];
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    if (32 * g >= P.pairs) break;
+    const int p = 32 * g + lane;
+    if (id[g] >= 0) B->token[B->row0[j[g]] + rank[g]] = (uint8_t)(p / P.K);
+    if (P.pos && blockIdx.x == 0 && p < P.pairs) P.pos[p] = id[g] >= 0 ? j[g] * kMxRows + rank[g] : -1;
+  }
+}
+
 enum : int { kModeF32 = 0, kModeF16 = 1, kModeBF16 = 2, kModeGated = 3 };
 
 // QT >= 0: the tokens come unquantised, as QT, at most kFewTokens of them in one
@@ -406,18 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   }
   if (!P.early) pdl_wait();
   pdl_trigger();
-  if (P.ids && warp == 3) {  // the pairs that have an expert
-    const int id = lane < P.pairs ? P.ids[lane] : -1;
-    const bool has = (unsigned)id < (unsigned)P.E;
-    const unsigned all = __ballot_sync(0xffffffffu, has);
-    if (has) {
-      const int j = __popc(all & ((1u << lane) - 1));
-      B->row0[j] = lane;
-      B->count[j] = id;
-    }
-    if (lane == 0) B->first[0] = __popc(all);
-    if (id >= P.E && blockIdx.x == 0) set_error(P.err, kDevBadExpert);
-  }
+  if (P.ids && warp == 3) sort_few(P, B, lane);
   if (P.offsets && warp == 3) {  // token tiles before each expert
     constexpr int kPer = kMaxExperts / 32;
     int c[kPer], s = 0;
@@ -448,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
   else __syncthreads();
   fence_after();
   const uint32_t tmem = B->tmem_base;
-  const int n_units = (P.ids       ? B->first[0]
+  const int n_units = (P.ids       ? B->experts
                        : P.offsets ? B->first[P.E]
                                    : (P.n_tokens + S::kTokens - 1) / S::kTokens) *
                       (kPair ? (P.w_tiles + 1) / 2 : P.w_tiles);
@@ -623,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       else ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + a * S::kTokens + U.col;
+      const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + a * S::kTokens;
       uint32_t r[32];
       if constexpr (MODE == kModeGated) {
         // 32 tokens at a time: all rows to shared memory (rows 0..63 gate,
@@ -631,10 +719,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
         const int nba = mx_blocks(P.n_out);
         float* x = ex + grp * (kMxRows * kExPitch);
         const int half = lane & 1, t = (q & 1) * 16 + (lane >> 1), b = q >> 1, blk = U.wt * 2 + b;
-        const float* xg = x + (32 * b + 16 * half) * kExPitch + t;
+        const float* xg = x + (32 * b + 16 * half) * kExPitch;
         const size_t act_tile = mx_tile_bytes(nba);
         for (int c0 = 32 * grp; c0 < U.n; c0 += 64) {
-          tmem_ld32(acc + c0, r);
+          // of unquantised tokens all were multiplied: each pair takes its own's column
+          tmem_ld32(acc + (QT >= 0 ? 0 : c0), r);
+          const int col = QT < 0 ? t : c0 + t < U.n ? B->token[U.list + c0 + t] : 0;
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[(32 * q + lane) * kExPitch + i] = __uint_as_float(r[i]);
@@ -643,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
           uint32_t amax = 0;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            v[i] = geglu(xg[i * kExPitch], xg[(64 + i) * kExPitch]);
+            v[i] = geglu(xg[i * kExPitch + col], xg[(64 + i) * kExPitch + col]);
             amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
           }
           amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -800,17 +890,17 @@ cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long 
   }
 }
 
-// A few pairs of tokens that a CTA can quantise itself, and no more of them
-// than experts: then hardly two share one, and sorting them saves nothing.
-// The layer of 128 experts, top-8, H = 2816, I = 704, unsorted in three
-// launches against sorted in five: 1 token 12.9 / 24.1 us, 2: 15.9 / 26.9,
-// 3: 17.7 / 29.8, 4: 23.7 / 30.4.
-bool mx4_few_pairs(int T, int K, int E, int H) {
-  return (long long)T * K <= std::min(32, E) && mx4_few_tokens(T, H);
+// Tokens that a CTA can quantise itself, and pairs that one warp sorts.  The layer
+// of 128 experts, top-8, H = 2816, I = 704, so in three launches against sorted
+// and gathered by launches of their own, five in all: 1 token 12.9 / 22.5 us, 2:
+// 16.0 / 27.4, 4: 23 / 33, 8: 38 / 45, 12: 49 / 54, 16: 56 / 61.
+bool mx4_few_pairs(int T, int K, int H) {
+  return T <= mx::kFewTokens && H <= mx::kFewCols && T * K <= mx::kFewPairs;
 }
 
-cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids, int T,
-                                   int K, int E, int H, int I, uint8_t* act, int* err, cudaStream_t s) {
+cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids,
+                                   int32_t* pos, int T, int K, int E, int H, int I, uint8_t* act, int* err,
+                                   cudaStream_t s) {
   mx::Params P{};
   P.w = w;
   P.E = E;
@@ -821,13 +911,14 @@ cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, lo
   P.act = act;
   P.err = err;
   P.ids = ids;
+  P.pos = pos;
   P.pairs = T * K;
   P.K = K;
   P.raw = x;
   P.ldx = ldx;
   P.cols = H;
   P.raw_vec = ((uintptr_t)x & 15) == 0 && (size_t)ldx * elem_bytes(type) % 16 == 0;
-  const long long units = (long long)T * K * P.w_tiles;
+  const long long units = (long long)std::min(E, T * K) * P.w_tiles;
   switch (type) {
     case kF32: return mx::launch<mx::kModeGated, false, kF32>(P, units, s);
     case kF16: return mx::launch<mx::kModeGated, false, kF16>(P, units, s);
@@ -851,7 +942,7 @@ cudaError_t launch_mx4_few_down(const uint8_t* w, const uint8_t* act, const int3
   P.pairs = T * K;
   P.K = K;
   P.early = 1;  // ids and weights are older than the launch before
-  return mx::launch<mx::kModeF32, false>(P, (long long)T * K * P.w_tiles, s);
+  return mx::launch<mx::kModeF32, false>(P, (long long)std::min(E, T * K) * P.w_tiles, s);
 }
 
 }  // namespace mrml

@@ -317,10 +317,10 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
   const ExpertsWs w = carve_experts(workspace, H, I, E, K, T);
   const cudaStream_t s = (cudaStream_t)stream;
   const long long pairs = (long long)T * K;
-  if (mrml::mx4_few_pairs(T, K, E, H)) {  // three launches: nothing is sorted or gathered
-    MRML_LAUNCH(mrml::launch_mx4_few_gate_up(type, gate_up, x, ldx, ids, T, K, E, H, I, w.act, w.sort.status, s));
+  if (mrml::mx4_few_pairs(T, K, H)) {  // three launches: no sort, no gather
+    MRML_LAUNCH(mrml::launch_mx4_few_gate_up(type, gate_up, x, ldx, ids, w.pos, T, K, E, H, I, w.act, w.sort.status, s));
     MRML_LAUNCH(mrml::launch_mx4_few_down(down, w.act, ids, T, K, E, H, I, w.y, w.sort.status, s));
-    MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, nullptr, probs, ids, E, down_scale, out, ldo, H, K, T, s));
+    MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
     return MRML_OK;
   }
   MRML_LAUNCH(mrml::launch_sort(ids, w.offsets, w.counts, w.pos, mrml::mx4_flat_bytes(H, K, T) ? w.pair : nullptr,
@@ -330,7 +330,7 @@ int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, 
                                     w.act, pairs, true, w.sort.status, s));
   MRML_LAUNCH(mrml::launch_mx4_gemm(MRML_F32, down, w.act, w.offsets, w.counts, E, 0, H, I, false, w.y, H,
                                     nullptr, pairs, true, w.sort.status, s));
-  MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, E, down_scale, out, ldo, H, K, T, s));
+  MRML_LAUNCH(mrml::launch_combine_rows(type, w.y, w.pos, probs, ids, down_scale, out, ldo, H, K, T, s));
   return MRML_OK;
 }
 

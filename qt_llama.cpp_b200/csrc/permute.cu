@@ -202,13 +202,12 @@ __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, l
 // weights are read once for all columns.  Bound by memory: 65536 f32 rows of
 // 2816 into 8192 bf16 tokens (785 MB) 120 us, 6.5 TB/s; bf16 rows (415 MB) 70 us,
 // 5.9 TB/s (one vector per thread and CTA: 129 and 75 us).  The weight of slot k is probs[t,k]
-// (1 without probs) times scale[ids[t,k]] (with scale).  Without pos, pair p's
-// row is 128 p if its id is one of n_experts.
+// (1 without probs) times scale[ids[t,k]] (with scale).
 template <int TYPE_IN, int TYPE, bool VEC>
 __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE_IN>::T* __restrict__ rows,
                                                         const int32_t* __restrict__ pos,
                                                         const float* __restrict__ probs,
-                                                        const int32_t* __restrict__ ids, int n_experts,
+                                                        const int32_t* __restrict__ ids,
                                                         const float* __restrict__ scale,
                                                         typename Elem<TYPE>::T* __restrict__ out, long long ldo,
                                                         int H, int K) {
@@ -225,11 +224,7 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       at[j] = -1;
-      if (k0 + j < K) {
-        const int p = (int)t * K + k0 + j;
-        if (pos) at[j] = __ldg(pos + p);
-        else if ((unsigned)__ldg(ids + p) < (unsigned)n_experts) at[j] = p * kMxRows;
-      }
+      if (k0 + j < K) at[j] = __ldg(pos + t * K + k0 + j);
       w[j] = k0 + j < K && probs ? __ldg(probs + t * K + k0 + j) : 1.f;
       if (scale && at[j] >= 0) w[j] *= __ldg(scale + __ldg(ids + t * K + k0 + j));
     }
@@ -412,7 +407,7 @@ cudaError_t launch_permute(int type, const void* x, long long ldx, const int32_t
 
 namespace {
 template <int TI, int TO>
-cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* probs, const int32_t* ids, int E,
+cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* probs, const int32_t* ids,
                          const float* scale, void* out, long long ldo, int H, int K, int T, cudaStream_t s) {
   using I = typename Elem<TI>::T;
   using O = typename Elem<TO>::T;
@@ -421,8 +416,8 @@ cudaError_t unpermute_as(const void* rows, const int32_t* pos, const float* prob
   const int v = vec ? Elem<TI>::kVec : 1, most = (H + 128 * v - 1) / (128 * v);
   const int parts = std::max(1, std::min(most, 4 * tc_num_sms() / std::max(1, T)));
   const dim3 grid(T, parts), block(128);
-  return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, E, scale, (O*)out, ldo, H, K)
-             : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, E, scale, (O*)out, ldo, H, K);
+  return vec ? launch_pdl(unpermute_kernel<TI, TO, true>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K)
+             : launch_pdl(unpermute_kernel<TI, TO, false>, grid, block, 0, s, (const I*)rows, pos, probs, ids, scale, (O*)out, ldo, H, K);
 }
 
 template <int TYPE>
@@ -441,19 +436,19 @@ cudaError_t unpermute_grad_as(const void* dout, long long ldd, const void* rows,
 cudaError_t launch_unpermute(int type, const void* rows, const int32_t* pos, const float* probs, void* out,
                              long long ldo, int H, int K, int T, cudaStream_t s) {
   switch (type) {
-    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, nullptr, 0, nullptr, out, ldo, H, K, T, s);
-    case kF16: return unpermute_as<kF16, kF16>(rows, pos, probs, nullptr, 0, nullptr, out, ldo, H, K, T, s);
-    default: return unpermute_as<kBF16, kBF16>(rows, pos, probs, nullptr, 0, nullptr, out, ldo, H, K, T, s);
+    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
+    case kF16: return unpermute_as<kF16, kF16>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
+    default: return unpermute_as<kBF16, kBF16>(rows, pos, probs, nullptr, nullptr, out, ldo, H, K, T, s);
   }
 }
 
 cudaError_t launch_combine_rows(int type, const float* rows, const int32_t* pos, const float* probs,
-                                const int32_t* ids, int E, const float* scale, void* out, long long ldo, int H, int K, int T,
+                                const int32_t* ids, const float* scale, void* out, long long ldo, int H, int K, int T,
                                 cudaStream_t s) {
   switch (type) {
-    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, ids, E, scale, out, ldo, H, K, T, s);
-    case kF16: return unpermute_as<kF32, kF16>(rows, pos, probs, ids, E, scale, out, ldo, H, K, T, s);
-    default: return unpermute_as<kF32, kBF16>(rows, pos, probs, ids, E, scale, out, ldo, H, K, T, s);
+    case kF32: return unpermute_as<kF32, kF32>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
+    case kF16: return unpermute_as<kF32, kF16>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
+    default: return unpermute_as<kF32, kBF16>(rows, pos, probs, ids, scale, out, ldo, H, K, T, s);
   }
 }
 

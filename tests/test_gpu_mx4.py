@@ -400,10 +400,13 @@ LAYERS = [
     (2048, 2, 16, 256, 128, 0.0, None),
     (700, 4, 8, 416, 352, 0.1, None), (1500, 2, 5, 320, 96, 0.0, 4), (900, 8, 16, 264, 200, 0.2, None),
     (4100, 4, 8, 1088, 700, 0.1, None), (3000, 8, 7, 1040, 333, 0.0, None),
-    # few enough pairs to go unsorted: dropped slots, all dropped, slots that share an expert, the largest
+    # few enough pairs for three launches: dropped slots, all dropped, slots that share an expert, the largest
     (1, 8, 128, 2816, 704, 0.0, None), (1, 8, 9, 96, 40, 0.4, None), (2, 4, 8, 320, 100, 1.0, None),
     (3, 4, 16, 1001, 70, 0.0, 5), (4, 8, 32, 2816, 96, 0.1, None), (16, 2, 61, 704, 130, 0.2, None),
     (1, 32, 64, 8192, 64, 0.0, None),
+    (16, 8, 128, 1001, 70, 0.2, None), (16, 8, 8, 320, 100, 0.0, 5), (2, 64, 256, 96, 40, 0.3, None),
+    (15, 8, 12, 2816, 96, 0.1, None), (9, 14, 60, 96, 65, 0.5, None), (16, 8, 16, 8192, 33, 0.0, None),
+    (17, 2, 16, 320, 64, 0.1, None),
     # large batches, more than 8 slots
     (2048, 8, 16, 1024, 64, 0.0, None), (6000, 8, 9, 600, 96, 0.05, None), (1500, 12, 24, 1001, 40, 0.3, None),
     (3200, 8, 16, 1088, 96, 0.1, None), (2500, 12, 24, 1001, 40, 0.3, None),
