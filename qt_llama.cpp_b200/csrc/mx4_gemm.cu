@@ -625,13 +625,15 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
         }
       }
       // Whatever happened, every copy lands before the block gives up its
-      // shared memory.
+      // shared memory; and so do the signals that the last stages are free
+      // (unless the walk ended early: those stages may never be).
       for (int i = 0; i < min(issued, kStages); ++i) {
         if (--R.s < 0) {
           R.s = kStages - 1;
           R.ph ^= 1;
         }
         mbar_wait_bounded(&B->full[R.s], R.ph, nullptr);
+        ok = ok && mbar_wait_bounded(&B->empty[R.s], R.ph, nullptr);
       }
     }
   } else if (warp == 1 && rank == 0) {
@@ -692,6 +694,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
           }
         }
       }
+      // The first CTA's commits signal barriers of this one too, and an
+      // arrival must not reach a CTA that has left: the last of them, which
+      // the first CTA commits on every path, is waited for here as there.
+      mbar_wait_bounded(&B->drain, 0, nullptr);
     }
   } else if (warp >= 4) {
     // Two groups of four warps; a group's warp q reads the lanes 32q..32q+31
