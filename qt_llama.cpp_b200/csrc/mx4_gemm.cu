@@ -190,14 +190,26 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrives on the first CTA's barrier at the same offset.  What it reports (a
-// stage's copies, an accumulator's reads) has completed by then; no memory of
-// this thread's own is handed over, so the arrival needs no release over the
-// cluster, which took 900 cycles and bounded the pair's chunk rate.
+// Arrives on the first CTA's barrier at the same offset.
+// ... with what this CTA's copies have brought to its shared memory, which the
+// first CTA's MMAs read: this thread has acquired it from the copies' own
+// barrier and passes it on by a release over the cluster.  Only shared memory
+// changes hands, so the fence is restricted to that; `arrive.release.cluster`,
+// which covers global memory too, takes 900 cycles, longer than a chunk's MMAs
+// (8192^3: 333 us against 200).
+__device__ __forceinline__ void release_to_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// ... and after reads of tensor memory, which the tcgen05 fences on the two
+// sides of the barrier order; no memory changes hands, so it is relaxed.
 __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 
@@ -687,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
       for (U.start(P, B); U.u < n_units && ok; U.u += step) {
         for (int c = 0; c < chunks; ++c) {
           if (!(ok = wait_at(full0 + 8 * s, ph, B, P.err))) break;
-          arrive_leader(&B->peer_full[s]);
+          release_to_leader(&B->peer_full[s]);
           if (++s == kStages) {
             s = 0;
             ph ^= 1;

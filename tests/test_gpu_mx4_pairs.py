@@ -51,3 +51,20 @@ def test_nothing_of_a_pair_outlives_it(cuda, moe, M, N, K):
         graph.replay()
         assert torch.equal(out, first) and torch.equal(few, first_few)
     assert moe.device_status(ws)[0] == 0 and moe.device_status(ws2)[0] == 0
+
+
+@pytest.mark.parametrize("M,N,K", PAIRED)
+def test_a_pair_reads_what_has_landed(cuda, moe, M, N, K):
+    """Two products of one shape in turn, so that a stage read before its copy had landed in either CTA would hold the
+    other product's operands (or another unit's)."""
+    runs = [product(moe, cuda, M, N, K, seed) for seed in (3, 4)]
+    first = []
+    for (x, w), run, out, _ in runs:
+        run()
+        check_product(out, mx4_values(x), mx4_values(w), torch.bfloat16)
+        first.append(out.clone())
+    for _ in range(40):
+        for _, run, out, _ in runs:
+            run()
+        assert all(torch.equal(r[2], f) for r, f in zip(runs, first))
+    assert all(moe.device_status(r[3])[0] == 0 for r in runs)
