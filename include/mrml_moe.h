@@ -393,7 +393,9 @@ int mrml_moe_sorted_rows(int E, int K, int T, int align);
  * offset a multiple of `align`.  offsets has E + 1 entries (the last: the
  * rows in use), counts E, pos T*K (the pair's row, or -1), pair
  * mrml_moe_sorted_rows(E, K, T, align) (the row's pair, or -1 for padding and
- * past the end).  A negative id marks a slot without an expert; an id of E or
+ * past the end); entries of a longer array past those are not written, so
+ * they are no rows for mrml_moe_permute or mrml_moe_unpermute_grad unless the
+ * caller sets them to -1.  A negative id marks a slot without an expert; an id of E or
  * more is skipped too and sets MRML_ERR_BAD_EXPERT_ID in the workspace
  * (mrml_moe_device_status).  E <= 256, K <= 64, T*K <= 2^26.  Workspace:
  * clear it once with mrml_moe_workspace_init. */

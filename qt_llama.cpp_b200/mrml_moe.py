@@ -484,14 +484,21 @@ def new_sort_workspace(E, K, T, device=None):
 
 
 def sort(ids, offsets, counts, pos, pair, E, K, T, align, ws, stream=None):
-    """mrml_moe_sort: the (token, slot) pairs in expert order."""
+    """mrml_moe_sort: the (token, slot) pairs in expert order.  A longer `pair`
+    (one sized for more tokens) has no pair in its further rows."""
     _check_ints(ids, offsets, counts, pos, pair)
     assert ids.numel() == T * K and pos.numel() == T * K
     assert offsets.numel() == E + 1 and counts.numel() == E
-    assert pair.numel() >= sorted_rows(E, K, T, align)
+    n = sorted_rows(E, K, T, align)
+    assert pair.numel() >= n
     _check("mrml_moe_sort",
            load_library().mrml_moe_sort(_ptr(ids), _ptr(offsets), _ptr(counts), _ptr(pos), _ptr(pair), E, K, T, align,
                                         _ptr(ws), ws.numel(), _stream_ptr(stream)))
+    if pair.numel() > n:  # the library writes n rows: what an earlier, larger batch left must not be taken for pairs
+        import torch
+
+        with torch.cuda.stream(stream):
+            pair.view(-1)[n:].fill_(-1)
 
 
 def permute(x, pair, rows, H, K, stream=None):
