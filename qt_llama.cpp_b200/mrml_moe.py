@@ -449,6 +449,17 @@ def _ld(t) -> int:
     return t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]
 
 
+def _folded_ld(t) -> int:
+    """Row stride in elements of a tensor of any number of axes, all its rows in order, whose leading axes lie in
+    memory as one (a slice between two longer axes does not)."""
+    if t.dim() <= 2 or t.is_contiguous():
+        return _ld(t)
+    assert t.stride(-1) == 1 or t.shape[-1] == 1, "columns must be contiguous"
+    axes = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    assert all(s == n1 * s1 for (_, s), (n1, s1) in zip(axes, axes[1:])), "leading axes must fold into one"
+    return axes[-1][1] if axes else t.shape[-1]
+
+
 def _check_ints(*tensors):
     i32 = (_torch_types or _types())[1]
     for t in tensors:
@@ -502,11 +513,11 @@ def sort(ids, offsets, counts, pos, pair, E, K, T, align, ws, stream=None):
 
 
 def permute(x, pair, rows, H, K, stream=None):
-    """mrml_moe_permute: rows[r] = x[pair[r] / K] (zero where pair[r] is -1)."""
+    """mrml_moe_permute: rows[r] = x[pair[r] / K] (zero where pair[r] is -1); x [..][H], its leading axes as one."""
     _check_ints(pair)
     assert x.shape[-1] == H and rows.shape == (pair.numel(), H) and rows.is_contiguous() and rows.dtype == x.dtype
     _check("mrml_moe_permute",
-           load_library().mrml_moe_permute(_float_type(x), _ptr(x), _ld(x), _ptr(pair), _ptr(rows), H, K,
+           load_library().mrml_moe_permute(_float_type(x), _ptr(x), _folded_ld(x), _ptr(pair), _ptr(rows), H, K,
                                            pair.numel(), _stream_ptr(stream)))
 
 

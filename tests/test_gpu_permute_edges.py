@@ -37,3 +37,26 @@ def test_buffers_of_a_larger_batch_serve_a_smaller_one(cuda, moe, few, align):
         drows, dprobs = torch.full_like(rows, 9.0), torch.empty(few, K, device=cuda)
         moe.unpermute_grad(x, rows, pos, pair, None, drows, dprobs, H, K, few)
         assert torch.equal(drows, want)
+
+
+def test_views_with_more_axes(cuda, moe):
+    """[batch][length][H] views: those whose rows lie at one stride are read as they are, others are refused."""
+    B, L, K, E, H = 5, 9, 2, 8, 24
+    base = torch.randn(B, L, 2 * H, device=cuda)
+    views = {
+        "whole": base, "columns": base[:, :, :H], "last": base[:, -1:, :], "one batch": base[1:2, 2:7, H:],
+        "every second batch": base[::2, 3:4], "one row": base[3:4, 4:5, 3:], "flat": base[:, 2],
+    }
+    for name, x in views.items():
+        T, h = x[..., 0].numel(), x.shape[-1]
+        (_, _, _, pair), _ = run_sort(moe, cuda, routing(T, T, K, E), E, 1)
+        rows = torch.full((pair.numel(), h), 9.0, device=cuda)
+        moe.permute(x, pair, rows, h, K)
+        assert torch.equal(rows, x.reshape(T, h)[pair.long() // K]), name
+    for x in (base[:, :4], base[:, ::2], base.transpose(0, 1), base[:, :, ::2]):
+        T, h = x[..., 0].numel(), x.shape[-1]
+        (_, _, _, pair), _ = run_sort(moe, cuda, routing(T, T, K, E), E, 1)
+        rows = torch.full((pair.numel(), h), 9.0, device=cuda)
+        with pytest.raises(AssertionError):
+            moe.permute(x, pair, rows, h, K)
+        assert (rows == 9.0).all()
