@@ -193,7 +193,14 @@ int mrml_moe_unpermute_grad(int type, const void* dout, int64_t lddout, const vo
   MRML_TRY(check_tokens(type, H, K, T));
   if (lddout < H || n_rows < 0) return MRML_ERR_INVALID_ARGUMENT;
   if (n_rows > kMaxRows) return MRML_ERR_UNSUPPORTED;
-  if (T == 0 || (!drows && !dprobs)) return MRML_OK;
+  if (T == 0) {  // no pairs: every row is one without
+    if (!drows || n_rows == 0) return MRML_OK;
+    if (!elem_aligned(drows, type)) return MRML_ERR_INVALID_ARGUMENT;
+    MRML_TRY(mrml::check_device());
+    return mrml::cuda_status(
+        cudaMemsetAsync(drows, 0, (size_t)n_rows * H * mrml::elem_bytes(type), (cudaStream_t)stream));
+  }
+  if (!drows && !dprobs) return MRML_OK;
   if (n_rows < T * K && drows) return MRML_ERR_INVALID_ARGUMENT;
   if (!dout || !pos || (drows && !pair) || (dprobs && !rows)) return MRML_ERR_INVALID_ARGUMENT;
   if (!elem_aligned(dout, type) || !elem_aligned(rows, type) || !elem_aligned(drows, type)) return MRML_ERR_INVALID_ARGUMENT;

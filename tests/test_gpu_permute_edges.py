@@ -60,3 +60,22 @@ def test_views_with_more_axes(cuda, moe):
         with pytest.raises(AssertionError):
             moe.permute(x, pair, rows, h, K)
         assert (rows == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_an_empty_batch_clears_the_rows(cuda, moe, dtype):
+    """No tokens, and a row buffer kept at its size: all its rows are without a pair, so their gradient is zero."""
+    K, E, H, n = 2, 8, 33, 70
+    i32 = dict(dtype=torch.int32, device=cuda)
+    pos, pair = torch.empty(0, K, **i32), torch.full((n,), 3, **i32)
+    ids, ws = torch.empty(0, K, **i32), moe.new_sort_workspace(E, K, 0, cuda)
+    moe.sort(ids, torch.empty(E + 1, **i32), torch.empty(E, **i32), pos, pair, E, K, 0, 1, ws)
+    assert (pair == -1).all()
+    rows, buf = torch.ones(n, H, dtype=dtype, device=cuda), torch.full((n + 2, H), 5.0, dtype=dtype, device=cuda)
+    drows, probs = buf[1:-1], torch.empty(0, K, device=cuda)
+    moe.unpermute_grad(torch.empty(0, H, dtype=dtype, device=cuda), rows, pos, pair, probs, drows,
+                       torch.empty(0, K, device=cuda), H, K, 0)
+    assert (drows == 0).all() and (buf[0] == 5).all() and (buf[-1] == 5).all()
+    # without a row gradient there is nothing to do
+    moe.unpermute_grad(torch.empty(0, H, dtype=dtype, device=cuda), rows, pos, pair, probs, None,
+                       torch.empty(0, K, device=cuda), H, K, 0)
