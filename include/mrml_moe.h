@@ -91,7 +91,11 @@ int mrml_moe_workspace_init(void *workspace, size_t workspace_bytes, mrml_stream
  * semantics of model.rs:1804-1829.  Logits, ids and probs equal the
  * reference CPU path's bit for bit (sequential f32 dot products, glibc's
  * expf).  The workspace is only checked for size and may be shared with
- * mrml_moe_experts. */
+ * mrml_moe_experts.  W (here and wherever a router runs) may be read before
+ * this library's call right before it on the stream has finished: W may be
+ * the result of a permutation or MXFP4 operator, of a copy or of another
+ * kernel, but not that of the layer's own calls (mrml_moe_forward, _experts,
+ * _ffn_*, _dense_ffn, _geglu, _rms_norm) without one of those in between. */
 int mrml_moe_router(const float *W, const float *x, float *logits, int32_t *ids, float *probs, int H, int E, int K,
                     int T, void *workspace, size_t workspace_bytes, mrml_stream_t stream);
 

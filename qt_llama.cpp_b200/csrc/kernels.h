@@ -50,8 +50,15 @@ inline cudaError_t ensure_smem(Kern k, size_t bytes, SmemOptIn& c) {
 // while the previous kernel on the stream finishes (its CTAs run their
 // prologue, then wait in pdl_wait() for the previous grid to complete and
 // its writes to be visible).  Every kernel of the library calls pdl_wait()
-// before its first read of anything an earlier kernel wrote, and
-// pdl_trigger() once its own CTAs are running.
+// before its first read of anything the launch before may have written or
+// let be written at the same time, and most call pdl_trigger() once their own
+// CTAs run.  Some read without waiting what they hold to be older:
+//   the router's kernels        the router weights
+//   the GGUF products           weights and work units
+//   the MXFP4 products `early`  weights, ids, unit list (launch_mx4_gemm)
+// So a kernel whose result a caller may pass as one of these does not call
+// pdl_trigger(): what follows it starts when it has completed.  That holds for
+// all float results of the permutation and MXFP4 operators.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                               Args... args) {

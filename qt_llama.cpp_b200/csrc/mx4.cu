@@ -244,8 +244,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t* __re
                                                              int vec) {
   using E = Elem<TYPE>;
   constexpr int V = E::kVec, kLanes = 128 / V, kStep = 32 / kLanes;  // lanes per row, rows at a time
-  pdl_wait();
-  pdl_trigger();
+  pdl_wait();  // no early start for the next launch, which may read dst without waiting (kernels.h)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nx = (cols + 127) / 128, m = blockIdx.y;
   const int tiles = (rows + kMxRows - 1) / kMxRows, tile = (int)(blockIdx.x / nx) >> 1;

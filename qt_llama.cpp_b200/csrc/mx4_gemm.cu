@@ -110,6 +110,9 @@ struct Params {
   // one start only after its own predecessors had completed: then the unit
   // list and the weights need not wait for it.
   int early;
+  // `out` is the caller's: the next launch may read it without waiting
+  // (kernels.h), and does not start early.
+  int last;
 };
 
 struct __align__(8) Bars {
@@ -516,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_kernel(const Params P) {
     }
   }
   if (!P.early) pdl_wait();
-  pdl_trigger();
+  if (!P.last) pdl_trigger();
   if (P.ids && warp == 3) sort_few(P, B, lane);
   if (P.offsets && warp == 3) {  // token tiles before each expert
     constexpr int kPer = kMaxExperts / 32;
@@ -865,6 +868,7 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   P.ldo = ldo;
   P.act = act;
   P.err = err;
+  P.last = offsets == nullptr;  // of the expert layer's products, both are read by launches of its own
   const int mode = gated ? mx::kModeGated : type == kF32 ? mx::kModeF32 : type == kF16 ? mx::kModeF16 : mx::kModeBF16;
   // Pairs of CTAs pay where there are enough units for several waves of them,
   // tokens to fill their tiles, and a sum long enough to be bound by the
@@ -897,6 +901,7 @@ cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long 
   P.out = out;
   P.ldo = ldo;
   P.err = err;
+  P.last = 1;
   P.raw = x;
   P.ldx = ldx;
   P.cols = cols;

@@ -8,6 +8,10 @@
 //   unpermute's gradients
 //              drows[pos[t,k]] = w[t,k] dout[t],  dw[t,k] = <dout[t], rows[pos[t,k]]>
 // Sums run in f32 in slot order and are rounded once.
+//
+// The kernels that write rows or tokens do not let the next launch start early:
+// a caller may use any of them as a matrix that a later kernel reads without
+// waiting (kernels.h).
 #include "../../include/mrml_moe.h"
 #include "kernels.h"
 #include "mx4.cuh"
@@ -171,7 +175,6 @@ __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, l
                                                       const int32_t* __restrict__ pair, T* __restrict__ rows, int H,
                                                       int K, int n_rows) {
   pdl_wait();
-  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (r >= n_rows) return;
@@ -216,7 +219,6 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
   constexpr int V = VEC ? EI::kVec : 1;  // values per vector: one 16-byte load of a row
   constexpr int S = 8;                   // slots at a time
   pdl_wait();
-  pdl_trigger();
   const long long t = blockIdx.x;
   int at[S];
   float w[S];
@@ -296,7 +298,6 @@ __global__ void __launch_bounds__(256) unpermute_grad_kernel(const typename Elem
   using E = Elem<TYPE>;
   using T = typename E::T;
   pdl_wait();
-  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int i0 = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int nv = H / E::kVec;

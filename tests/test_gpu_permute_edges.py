@@ -79,3 +79,57 @@ def test_an_empty_batch_clears_the_rows(cuda, moe, dtype):
     # without a row gradient there is nothing to do
     moe.unpermute_grad(torch.empty(0, H, dtype=dtype, device=cuda), rows, pos, pair, probs, None,
                        torch.empty(0, K, device=cuda), H, K, 0)
+
+
+@pytest.mark.parametrize("T", [1, 8])
+def test_router_weights_written_right_before(cuda, moe, T):
+    """Router weights that another operator of the library writes right before the router reads them, with fresh
+    contents each time, in a stream and in a graph.  The logits are one fixed chain of additions, so they equal those of
+    a settled copy."""
+    H, E, K, rounds = 2816, 128, 8, 24
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn(T, H, generator=g, device=cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    ws, mm = moe.new_workspace(32, 32, E, K, T, cuda), moe.new_mx4_matmul_workspace(E, H, 64, cuda)
+    W, codes = torch.zeros(E, H, device=cuda), moe.new_mx4(E, H, 1, cuda)
+    a, b = moe.new_mx4(E, 64, 1, cuda), moe.new_mx4(H, 64, 1, cuda)
+    moe.mx4_quantize(torch.randn(H, 64, generator=g, device=cuda), b, H, 64)
+    order = torch.randperm(E, generator=g, device=cuda).to(torch.int32)
+    base = torch.empty(E, H, device=cuda)
+
+    def by_dequantising(new, s):
+        moe.mx4_quantize(new, codes, E, H, stream=s)
+        moe.mx4_dequantize(codes, W, E, H, stream=s)
+
+    def by_product(new, s):
+        moe.mx4_quantize(new[:, :64], a, E, 64, stream=s)
+        moe.mx4_matmul(a, b, W, E, H, 64, mm, stream=s)
+
+    def by_gathering(new, s):
+        moe.permute(new, order, W, H, 1, stream=s)
+
+    def by_summing(new, s):
+        moe.unpermute(new, order, None, W, H, 1, E, stream=s)
+
+    s = torch.cuda.Stream()
+    for write in (by_dequantising, by_product, by_gathering, by_summing):
+        logits, ids, probs = torch.empty(T, E, device=cuda), torch.empty(T, K, **i32), torch.empty(T, K, device=cuda)
+        step = lambda: (write(base, s), moe.router(W, x, logits, ids, probs, H, E, K, T, ws, s))  # noqa: E731
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            step()
+        for i in range(rounds):
+            base.normal_(generator=g)
+            torch.cuda.synchronize()
+            if i % 2:
+                step()
+            else:
+                graph.replay()
+            torch.cuda.synchronize()
+            got = logits.clone(), ids.clone(), probs.clone()
+            settled = W.clone()
+            torch.cuda.synchronize()
+            moe.router(settled, x, logits, ids, probs, H, E, K, T, ws)
+            torch.cuda.synchronize()
+            assert all(torch.equal(u, v) for u, v in zip(got, (logits, ids, probs))), write.__name__
