@@ -241,9 +241,13 @@ cudaError_t launch_mx4_gather(int type, const void* x, long long ldx, const int3
 // 128); without: one matrix and n_tokens rows.  gated: the weights are in the
 // gated row order and the MXFP4 result act = gelu(gate) * up replaces out.
 // tokens: the rows that are expected in all (the choice of kernel and grid).
-// early: of the kernel launched right before, only x (and the last use of act)
-// matters, and that kernel waits for its own predecessor before it lets the
-// next start: the rest is read without waiting for it.
+// early: of the launch right before, only x (and the last use of act) matters;
+// the rest is read without waiting for it.  All of that rest must be older than
+// the nearest launch before that waits for its own predecessor before it lets
+// the next start (the gather, the quantisation); launches between that one and
+// this may be early products themselves, which let the next start at once.  So
+// in the expert layer the sort's results and the weights are complete before
+// the gather lets the gate/up product start, and with it the down product.
 cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const int32_t* offsets,
                             const int32_t* counts, int E, int n_tokens, int rows, int cols, bool gated, void* out,
                             long long ldo, uint8_t* act, long long tokens, bool early, int* err, cudaStream_t s);

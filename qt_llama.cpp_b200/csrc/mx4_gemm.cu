@@ -106,9 +106,9 @@ struct Params {
   long long ldx;
   int cols, raw_vec;
   // Nothing but the tokens (and, for the GeGLU's result, earlier readers of
-  // act) comes from the kernel right before this one, and that kernel let this
-  // one start only after its own predecessors had completed: then the unit
-  // list and the weights need not wait for it.
+  // act) comes from the kernel right before this one or runs beside it; the
+  // unit list and the weights are older than a launch that waited before it let
+  // its successors start (kernels.h), and need no wait here.
   int early;
   // `out` is the caller's: the next launch may read it without waiting
   // (kernels.h), and does not start early.
