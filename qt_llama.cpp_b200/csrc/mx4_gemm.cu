@@ -84,6 +84,11 @@ struct Shape {
   static constexpr int kStageBytes = kMxChunkBytes + kTokenScales + (kPair ? kTokens / 2 : kTokens) * kMxChunk * 16;
   static constexpr uint32_t kSf0 = 2 * kTokens, kSfCols = 8 + 8 * kTokenTiles;
   static_assert(kSf0 + kStages * kSfCols <= 512, "tensor memory has 512 columns");
+  // A unit's first row sets the column where its scales start in their group of
+  // four (Issue::shift); only even columns are supported, so units start at
+  // multiples of 64 rows (and with one token tile at that tile's start).
+  static_assert(kTokens % 64 == 0 && kMxRows % 64 == 0 && (kPair || kTokens % kMxRows == 0),
+                "units start at even columns of the token scales");
 };
 
 struct Params {
