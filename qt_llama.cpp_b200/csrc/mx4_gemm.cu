@@ -887,11 +887,16 @@ cudaError_t launch_mx4_gemm(int type, const uint8_t* w, const uint8_t* x, const 
   return mx::launch_mode<false>(mode, P, (tokens / 128 + std::min<long long>(E, tokens)) * P.w_tiles, s);
 }
 
-// About one block per quantising thread: 4 tokens of 2816 take 6.0 us in one
-// launch and 5.8 in two, 1 token 5.0 and 5.9, 16 tokens 7.9 and 5.9 (4224
-// outputs); 16 tokens of 704 4.6 and 4.6 (2816 outputs).
+// At most one block per quantising thread.  One launch against two, replayed in
+// graphs (us, blocks in brackets):
+//   704 -> 2816:   4 tokens (88) 4.4 / 4.9, 12 (264) 4.9 / 5.2, 16 (352) 5.4 / 5.2
+//   1024 -> 1024:  8 (256) 5.4 / 5.5, 12 (384) 5.8 / 5.5
+//   2816 -> 4224:  1 (88) 7.3 / 8.2, 3 (264) 7.7 / 8.3, 4 (352) 8.2 / 8.3, 6 (528) 8.3 / 7.8
+//   4096 -> 4096:  2 (256) 8.9 / 9.0, 3 (384) 9.4 / 9.0
+//   8192 -> 8192:  1 (256) 13.0 / 13.8, 2 (512) 13.6 / 13.8, 3 (768) 14.2 / 13.8
 bool mx4_few_tokens(int tokens, int cols) {
-  return tokens <= mx::kFewTokens && cols <= mx::kFewCols && (long long)tokens * mx_blocks(cols) <= 384;
+  return tokens <= mx::kFewTokens && cols <= mx::kFewCols &&
+         (long long)tokens * mx_blocks(cols) <= 32 * mx::kFewWarps;
 }
 
 cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long ldx, int n_tokens, int rows, int cols,

@@ -1,0 +1,27 @@
+"""MXFP4 operators on both sides of the rules that choose between their forms, and at values where they can go wrong.
+
+The bounds are test_gpu_mx4.py's: quantised values are exact, a product's error is bounded by its number of f32
+additions, the expert layer's by what those errors can do to its quantised activations."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_mx4 import check_product, mx4_values, quantize
+from test_gpu_permute import UNIT
+
+pytestmark = pytest.mark.gpu
+
+
+# tokens of K summed values: at most 320 blocks are quantised by the product itself, more by a launch of their own
+@pytest.mark.parametrize("dtype", list(UNIT))
+@pytest.mark.parametrize("T,N,K", [(14, 300, 704), (15, 300, 704), (10, 129, 1024), (11, 129, 1024), (1, 200, 8192),
+                                   (2, 200, 8192), (5, 130, 2048), (6, 130, 2048), (16, 257, 640), (16, 257, 641)])
+def test_linear_on_both_sides_of_its_rule(cuda, moe, T, N, K, dtype):
+    g = torch.Generator(device=cuda).manual_seed(T * K)
+    x, w = torch.randn(T, K, generator=g, device=cuda).to(dtype), torch.randn(N, K, generator=g, device=cuda).to(dtype)
+    out, ws = torch.full((T, N), 3.0, dtype=dtype, device=cuda), moe.new_mx4_linear_workspace(T, N, K, cuda)
+    moe.mx4_linear(x, quantize(moe, w), out, T, N, K, ws)
+    assert moe.device_status(ws)[0] == 0
+    check_product(out, mx4_values(x), mx4_values(w), dtype)
