@@ -923,12 +923,18 @@ cudaError_t launch_mx4_few(int type, const uint8_t* w, const void* x, long long 
   }
 }
 
-// Tokens that a CTA can quantise itself, and pairs that one warp sorts.  The layer
-// of 128 experts, top-8, H = 2816, I = 704, so in three launches against sorted
-// and gathered by launches of their own, five in all: 1 token 12.9 / 22.5 us, 2:
-// 16.0 / 27.4, 4: 23 / 33, 8: 38 / 45, 12: 49 / 54, 16: 56 / 61.
+// Pairs that one warp sorts, and tokens that a CTA quantises itself: up to 2048
+// blocks, as every CTA quantises them all.  Three launches against the five
+// with a sort and a gather of their own, each step with other experts' weights,
+// replayed in graphs (us):
+//   H 2816, I 704, 128 experts top-8:  1 token 15.6 / 25.2, 8 39.6 / 47.0, 16 (1408 blocks) 58.6 / 62.5
+//   H 1024, I 512, 16 top-2:           1 10.5 / 14.0, 16 13.2 / 15.5
+//   H 4096, I 1024, 256 top-4:         1 17.3 / 31.6, 16 (2048) 74.6 / 83.9
+//   H 5632, I 704, 32 top-4:           8 (1408) 35.6 / 37.8, 12 (2112) 44.2 / 43.1
+//   H 8192, I 512, 64 top-8:           8 (2048) 64.9 / 67.9, 12 (3072) 73.6 / 73.3, 16 86.6 / 83.7
+//   H 8192, I 2048, 16 top-2:          4 (1024) 43.8 / 45.4, 8 59.3 / 58.5, 16 81.2 / 75.6
 bool mx4_few_pairs(int T, int K, int H) {
-  return T <= mx::kFewTokens && H <= mx::kFewCols && T * K <= mx::kFewPairs;
+  return T <= mx::kFewTokens && H <= mx::kFewCols && T * K <= mx::kFewPairs && T * mx_blocks(H) <= 2048;
 }
 
 cudaError_t launch_mx4_few_gate_up(int type, const uint8_t* w, const void* x, long long ldx, const int32_t* ids,

@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_mx4 import check_product, mx4_values, quantize
+from test_gpu_mx4 import check_product, experts_case, experts_reference, mx4_values, quantize, run_experts
 from test_gpu_permute import UNIT
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +25,15 @@ def test_linear_on_both_sides_of_its_rule(cuda, moe, T, N, K, dtype):
     moe.mx4_linear(x, quantize(moe, w), out, T, N, K, ws)
     assert moe.device_status(ws)[0] == 0
     check_product(out, mx4_values(x), mx4_values(w), dtype)
+
+
+# few pairs: 16 tokens, 128 pairs and 2048 blocks are the most that take three launches
+@pytest.mark.parametrize("dtype", list(UNIT))
+@pytest.mark.parametrize("T,K,E,H,I", [(8, 8, 16, 8192, 33), (9, 8, 16, 8192, 33), (16, 8, 64, 4096, 40), (16, 2, 8, 4160, 40),
+                                       (16, 8, 8, 96, 64), (16, 9, 16, 96, 64), (2, 64, 128, 320, 33)])
+def test_layer_on_both_sides_of_its_rule(cuda, moe, T, K, E, H, I, dtype):
+    c = experts_case(T * K, T, K, E, H, I, dtype, cuda, 0.1)
+    out, ws = run_experts(moe, c, T, K, E, H, I)
+    assert moe.device_status(ws)[0] == 0
+    want, tol = experts_reference(c, T, K, E, H, I)
+    assert ((out.double() - want).abs() <= tol).all()
