@@ -415,14 +415,22 @@ cudaError_t launch_mx4_dequantize(int type, const uint8_t* src, void* out, long 
   }
 }
 
-// Pairs from which the gather runs in two steps.  The expert layer (H = 2816, 128
-// experts) in one and in two steps: 8192 pairs 126 and 135 us, 16384 191 and 193,
-// 20480 234 and 236, 32768 303 and 291, 49152 415 and 388.
-constexpr long long kGatherFlatPairs = 24576;
+// The gather runs in two steps where a token goes to several experts and the
+// rows are many: from 80 million gathered values.  The expert layer (us) in one
+// and in two steps, by pairs:
+//   H 2816, 128 experts top-8: 24576 pairs (69 M) 240 / 242, 32768 (92 M) 298 / 290, 65536 506 / 466
+//   H 8192, 64 top-8:          8192 (67 M) 211 / 220, 16384 (134 M) 368 / 349, 65536 1231 / 1060
+//   H 4096, 32 top-4:          16384 (67 M) 178 / 179, 24576 (101 M) 241 / 234
+//   H 1024, 16 top-2:          65536 (67 M) 261 / 264, 131072 (134 M) 512 / 505
+//   H 256, 128 top-8:          131072 (34 M) 145 / 145
+//   H 2816, 16 top-1:          65536 (185 M) 761 / 774, 131072 1503 / 1531
+constexpr long long kGatherFlatValues = 80'000'000;
+
+bool gather_flat(int H, int K, int T) { return K > 1 && (long long)T * K * H >= kGatherFlatValues; }
 
 size_t mx4_flat_bytes(int H, int K, int T) {
   const int nb = mx_blocks(H);
-  return (long long)T * K < kGatherFlatPairs ? 0 : (size_t)T * (nb * 16 + flat_scales(nb));
+  return gather_flat(H, K, T) ? (size_t)T * (nb * 16 + flat_scales(nb)) : 0;
 }
 
 namespace {
@@ -431,7 +439,7 @@ cudaError_t gather_as(const void* x, long long ldx, const int32_t* pos, const in
                       uint8_t* dst, uint8_t* flat, int T, int H, int K, int n_rows, cudaStream_t s) {
   using E = typename Elem<TYPE>::T;
   const int vec = vec_ok(x, ldx, 0, sizeof(E)), nb = mx_blocks(H);
-  if ((long long)T * K < kGatherFlatPairs) {
+  if (!gather_flat(H, K, T)) {
     const dim3 grid((unsigned)(((long long)T * ((nb + 31) / 32) + 7) / 8));
     return launch_pdl(mx4_gather_kernel<TYPE>, grid, 256, 0, s, (const E*)x, ldx, pos, dst, T, H, K, vec);
   }

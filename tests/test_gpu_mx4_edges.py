@@ -37,3 +37,26 @@ def test_layer_on_both_sides_of_its_rule(cuda, moe, T, K, E, H, I, dtype):
     assert moe.device_status(ws)[0] == 0
     want, tol = experts_reference(c, T, K, E, H, I)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+# from 80 million gathered values, and with more than one slot, the tokens are quantised before they are gathered
+@pytest.mark.parametrize("dtype", list(UNIT))
+@pytest.mark.parametrize("T,K,E,H,I,drop", [(10000, 8, 16, 1001, 40, 0.1), (9980, 8, 16, 1001, 40, 0.0), (6700, 12, 24, 1001, 33, 0.3),
+                                            (20100, 4, 9, 1000, 40, 0.0), (80100, 1, 5, 1000, 33, 0.1), (1300, 8, 8, 8192, 33, 0.05)])
+def test_large_layer_on_both_sides_of_its_rule(cuda, moe, T, K, E, H, I, drop, dtype):
+    c = experts_case(T + K, T, K, E, H, I, dtype, cuda, drop)
+    out, ws = run_experts(moe, c, T, K, E, H, I)
+    assert moe.device_status(ws)[0] == 0
+    want, tol = experts_reference(c, T, K, E, H, I)
+    assert ((out.double() - want).abs() <= tol).all()
+    again, _ = run_experts(moe, c, T, K, E, H, I, ws=ws)
+    assert torch.equal(again, out)
+
+
+def test_a_layer_workspace_serves_fewer_tokens(moe):
+    """Also where the two-step gather begins, which depends on the tokens' width."""
+    lib = moe.load_library()
+    for H, K in ((256, 8), (1001, 8), (2816, 8), (8192, 2), (8192, 1)):
+        at = 80_000_000 // (H * K)
+        sizes = [lib.mrml_moe_mx4_experts_workspace_bytes(H, 64, 16, K, T) for T in range(at - 20, at + 20)]
+        assert sizes == sorted(sizes)
