@@ -83,19 +83,31 @@ def serve(device, H=1024, I=512, E=16, K=2, batches=(1, 64, 2048)):
     return outs
 
 
+def sort_tokens(ids, E, ws):
+    """pos and pair of the tokens' experts, in tensors of their own: gradients need those of their own pass, and
+    autograd does not see the library write into a buffer that is used again."""
+    T, K = ids.shape
+    i32 = dict(dtype=torch.int32, device=ids.device)
+    offsets, counts = torch.empty(E + 1, **i32), torch.empty(E, **i32)
+    pos, pair = torch.empty(T, K, **i32), torch.empty(moe.sorted_rows(E, K, T), **i32)
+    moe.sort(ids.to(torch.int32).contiguous(), offsets, counts, pos, pair, E, K, T, 1, ws)
+    return pos, pair
+
+
 class Permuted(torch.autograd.Function):
     """Tokens gathered in expert order, and the gradient back to them."""
 
     @staticmethod
     def forward(ctx, x, pos, pair, H, K, T):
-        ctx.args = (pos, H, K, T)
+        ctx.save_for_backward(pos)
+        ctx.shape = (H, K, T)
         rows = torch.empty(pair.numel(), H, dtype=x.dtype, device=x.device)
         moe.permute(x, pair, rows, H, K)
         return rows
 
     @staticmethod
     def backward(ctx, drows):
-        pos, H, K, T = ctx.args
+        (pos,), (H, K, T) = ctx.saved_tensors, ctx.shape
         dx = torch.empty(T, H, dtype=drows.dtype, device=drows.device)
         moe.permute_grad(drows.contiguous(), pos, dx, H, K, T)
         return dx, None, None, None, None, None
@@ -106,16 +118,15 @@ class Unpermuted(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rows, probs, pos, pair, H, K, T):
-        ctx.save_for_backward(rows, probs)
-        ctx.args = (pos, pair, H, K, T)
+        ctx.save_for_backward(rows, probs, pos, pair)
+        ctx.shape = (H, K, T)
         out = torch.empty(T, H, dtype=rows.dtype, device=rows.device)
         moe.unpermute(rows, pos, probs, out, H, K, T)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        rows, probs = ctx.saved_tensors
-        pos, pair, H, K, T = ctx.args
+        (rows, probs, pos, pair), (H, K, T) = ctx.saved_tensors, ctx.shape
         drows, dprobs = torch.empty_like(rows), torch.empty_like(probs)
         moe.unpermute_grad(dout.contiguous(), rows, pos, pair, probs, drows, dprobs, H, K, T)
         return drows, dprobs, None, None, None, None, None
@@ -133,12 +144,13 @@ class Mx4Linear(torch.autograd.Function):
         moe.mx4_quantize_both(w, q[2], q[3], N, K)
         y = torch.empty(T, N, dtype=x.dtype, device=x.device)
         moe.mx4_matmul(q[0], q[2], y, T, N, K, moe.new_mx4_matmul_workspace(T, N, K, x.device))
-        ctx.q, ctx.shape = (q[1], q[3]), (T, N, K)
+        ctx.save_for_backward(q[1], q[3])
+        ctx.shape = (T, N, K)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        (T, N, K), (xt, wt), dev = ctx.shape, ctx.q, dy.device
+        (T, N, K), (xt, wt), dev = ctx.shape, ctx.saved_tensors, dy.device
         dy = dy.contiguous()
         d, dt = moe.new_mx4(T, N, 1, dev), moe.new_mx4(N, T, 1, dev)
         moe.mx4_quantize_both(dy, d, dt, T, N)
@@ -156,14 +168,11 @@ def train(device, T=512, H=256, E=8, K=2, steps=12, lr=0.15):
     x = torch.randn(T, H, generator=g, device=device)
     w = (0.02 * torch.randn(H, H, generator=g, device=device)).requires_grad_()
     router = (0.1 * torch.randn(E, H, generator=g, device=device)).requires_grad_()
-    i32 = dict(dtype=torch.int32, device=device)
-    offsets, counts = torch.empty(E + 1, **i32), torch.empty(E, **i32)
-    pos, pair = torch.empty(T, K, **i32), torch.empty(moe.sorted_rows(E, K, T), **i32)
     ws = moe.new_sort_workspace(E, K, T, device)
     losses = []
     for _ in range(steps):
         top, ids = torch.topk(x @ router.t(), K, dim=1)
-        moe.sort(ids.to(torch.int32), offsets, counts, pos, pair, E, K, T, 1, ws)
+        pos, pair = sort_tokens(ids, E, ws)
         rows = Mx4Linear.apply(Permuted.apply(x, pos, pair, H, K, T), w)
         out = Unpermuted.apply(rows, torch.softmax(top, 1), pos, pair, H, K, T)
         loss = (out - x).square().mean()
