@@ -31,7 +31,8 @@ long long rows_bound(int E, int K, int T, int align) {
   if (E <= 0 || K <= 0 || T < 0 || align <= 0 || align > 128) return -1;
   const long long pairs = (long long)T * K;
   if (pairs > kMaxPairs) return -1;
-  return pairs + std::min<long long>(E, pairs) * (align - 1);
+  const long long rows = pairs + std::min<long long>(E, pairs) * (align - 1);
+  return rows > kMaxRows ? -1 : rows;
 }
 
 // Shapes of the permutation entry points.
