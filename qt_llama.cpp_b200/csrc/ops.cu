@@ -114,6 +114,16 @@ int check_product(int type, int M, int N, int K) {
   return MRML_OK;
 }
 
+// Shapes of the expert layer.
+int check_experts(int type, int H, int I, int E, int K, int T) {
+  MRML_TRY(check_tokens(type, H, K, T));
+  if (I <= 0 || E <= 0) return MRML_ERR_INVALID_ARGUMENT;
+  if (E > kMaxExperts || I > kMaxCols) return MRML_ERR_UNSUPPORTED;
+  const long long n_rows = rows_bound(E, K, T, mrml::kMxRows);
+  if (n_rows < 0) return MRML_ERR_UNSUPPORTED;
+  return check_product(type, (int)n_rows, std::max(2 * I, H), std::max(H, I));
+}
+
 // `early`: a was written by the launch right before, b not (launch_mx4_gemm).
 int matmul(int type, const uint8_t* a, const uint8_t* b, void* out, int64_t ldo, int M, int N, int K, void* workspace,
            size_t workspace_bytes, bool early, mrml_stream_t stream) {
@@ -303,20 +313,15 @@ int mrml_moe_mx4_linear(int type, const void* x, int64_t ldx, const uint8_t* w, 
 }
 
 size_t mrml_moe_mx4_experts_workspace_bytes(int H, int I, int E, int K, int T) {
-  if (H <= 0 || I <= 0 || E > kMaxExperts || rows_bound(E, K, T, mrml::kMxRows) < 0) return 0;
-  return carve_experts(nullptr, H, I, E, K, T).bytes;
+  return check_experts(MRML_F32, H, I, E, K, T) == MRML_OK ? carve_experts(nullptr, H, I, E, K, T).bytes : 0;
 }
 
 int mrml_moe_mx4_experts(int type, const uint8_t* gate_up, const uint8_t* down, const int32_t* ids, const float* probs,
                          const float* down_scale, const void* x, int64_t ldx, void* out, int64_t ldo, int H, int I,
                          int E, int K, int T, void* workspace, size_t workspace_bytes, mrml_stream_t stream) {
-  MRML_TRY(check_tokens(type, H, K, T));
-  if (I <= 0 || E <= 0 || ldx < H || ldo < H) return MRML_ERR_INVALID_ARGUMENT;
-  if (E > kMaxExperts || I > 0x3fffff00) return MRML_ERR_UNSUPPORTED;
-  const long long n_rows = rows_bound(E, K, T, mrml::kMxRows);
-  if (n_rows < 0) return MRML_ERR_UNSUPPORTED;
+  MRML_TRY(check_experts(type, H, I, E, K, T));
+  if (ldx < H || ldo < H) return MRML_ERR_INVALID_ARGUMENT;
   if (T == 0) return MRML_OK;
-  MRML_TRY(check_product(type, (int)std::min<long long>(n_rows, 0x7fffff00), std::max(2 * I, H), std::max(H, I)));
   if (!gate_up || !down || !ids || !probs || !x || !out) return MRML_ERR_INVALID_ARGUMENT;
   if (!aligned16(gate_up) || !aligned16(down) || !elem_aligned(x, type) || !elem_aligned(out, type))
     return MRML_ERR_INVALID_ARGUMENT;
