@@ -133,3 +133,30 @@ def test_router_weights_written_right_before(cuda, moe, T):
             moe.router(settled, x, logits, ids, probs, H, E, K, T, ws)
             torch.cuda.synchronize()
             assert all(torch.equal(u, v) for u, v in zip(got, (logits, ids, probs))), write.__name__
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_non_finite_values_stay_where_they_belong(cuda, moe, dtype):
+    """Weights of dropped slots are not read as factors, and a token's non-finite values reach its own results only."""
+    T, K, E, H = 30, 3, 5, 72
+    ids = routing(4, T, K, E, 0.4)
+    ids[7], ids[8, 0], ids[9, 1] = -1, 2, 3  # a token without any slot, and two that have one
+    (_, _, pos, pair), _ = run_sort(moe, cuda, ids, E, 1)
+    none = pos < 0
+    probs = torch.rand(T, K, device=cuda).masked_fill(none, float("nan"))
+    rows = torch.ones(pair.numel(), H, dtype=dtype, device=cuda)
+    rows[(pair < 0)] = float("nan")
+    out = torch.full((T, H), 9.0, dtype=dtype, device=cuda)
+    moe.unpermute(rows, pos, probs, out, H, K, T)
+    assert torch.isfinite(out).all() and (out[7] == 0).all()
+    dout = torch.ones(T, H, dtype=dtype, device=cuda)
+    dout[7, 1], dout[8, 5], dout[9, 6] = float("nan"), float("inf"), float("nan")
+    drows, dprobs = torch.full_like(rows, 9.0), torch.full_like(probs, 9.0)
+    moe.unpermute_grad(dout, rows, pos, pair, probs, drows, dprobs, H, K, T)
+    token = torch.where(pair >= 0, pair // K, -1)
+    bad = torch.zeros_like(rows, dtype=torch.bool)
+    bad[token == 8, 5], bad[token == 9, 6] = True, True
+    assert torch.equal(~torch.isfinite(drows), bad) and (drows[pair < 0] == 0).all()
+    want = torch.zeros_like(none)
+    want[8], want[9] = ~none[8], ~none[9]
+    assert torch.equal(~torch.isfinite(dprobs), want) and (dprobs[none] == 0).all()
