@@ -49,8 +49,10 @@ __device__ __forceinline__ void store_block(uint8_t* tile, int nb, int r, int b,
 
 // A warp takes 8 rows x 4 blocks of a tile: each lane one block, so that a
 // row is read in 128 contiguous values and every 128-byte line of codes is
-// written whole.  TYPE < 0: GGUF blocks.  128 bf16 matrices of 1408 x 2816 (1285
-// MB) take 187 us, 6.9 TB/s.
+// written whole.  128 bf16 matrices of 1408 x 2816 (1285 MB) take 187 us, 6.9
+// TB/s.  TYPE < 0: GGUF blocks, read in their two-byte units (18 and 34 bytes,
+// so no wider load is aligned): Q4_0 (555 MB) 259 us, 2.1 TB/s, Q8_0 (809 MB) 265
+// us, 3.1 TB/s, once per model.
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const void* __restrict__ src, long long ldx,
                                                            long long mstride, uint8_t* __restrict__ dst, int rows,
@@ -94,8 +96,9 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const void* __restric
 // the two reads half the rows of two adjacent columns, so that 16-bit values
 // come in whole words, they share the columns' maxima, and half a block of
 // codes changes hands.  Both outputs are written in whole 128-byte lines.
-// Bound by instruction issue and shared memory rather than by DRAM: 22528 x
-// 2816 bf16 (194 MB) 43 us, 4.5 TB/s.
+// 22528 x 2816 bf16 (194 MB) 43 us, 4.5 TB/s, no unit at its limit: instruction
+// issue at 58 %, the load/store data pipe at 60 (33 of them shared memory), DRAM
+// at 44, with 46 % of the warps that an SM could hold.
 constexpr int kBothCols = 128;
 template <int TYPE>
 constexpr int kBothRows = TYPE == kF32 ? 64 : 128;  // of 48 KB of shared memory

@@ -37,11 +37,12 @@
 //
 // Measured (weights of a 128-expert layer, H = 2816, I = 704): 64 tokens' gate
 // and up product 40 us for 270 MB of weights and activations, 6.7 TB/s, the
-// copy rate; 8192 tokens' 155 us, 3.4 PFLOP/s, bound by shared memory (operands
-// in, operands read by the tensor cores, the GeGLU's exchange), and the down
-// product 158 us, bound by writing its 738 MB of f32 rows (5.4 TB/s over all its
-// DRAM traffic).  Dense bf16: 4096 x 4224 x 2816 27 us, 3.6 PFLOP/s, one and a
-// fraction of waves lost to rounding; 8192^3 200 us, 5.5 PFLOP/s.
+// copy rate; 8192 tokens' 155 us, 3.4 PFLOP/s, no unit at its limit (of 64 bytes
+// a cycle 41 copied in, the shared-memory pipe at 60 %: 34 for the tensor cores,
+// 26 for the GeGLU's exchange; the tensor pipe at 48 %), and the down product 158
+// us, bound by writing its 738 MB of f32 rows (5.4 TB/s over all its DRAM
+// traffic).  Dense bf16: 4096 x 4224 x 2816 27 us, 3.6 PFLOP/s, 374 units for 74
+// pairs, so five waves and a sixth of four units; 8192^3 200 us, 5.5 PFLOP/s.
 //
 // Scales live in tensor memory per shared-memory stage, so a stage's scales
 // are overwritten only after the MMAs that read them have completed.

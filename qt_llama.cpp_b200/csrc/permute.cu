@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(SortArgs a) {
 // order, while the tokens are read from L2 after their first use.  VEC: 16-byte
 // vectors (rows and strides aligned).  Bound by memory, seven eighths of it
 // writes: 65536 rows of 2816 bf16 (415 MB) 77 us, 5.4 TB/s; the streaming hint
-// on the stores is worth 7 % (85 us without), one on the loads nothing.
+// on the stores is worth 7 % (85 us without), one on the loads nothing.  Rows that
+// are not aligned go element by element: of 2815 bf16 172 us, f32 297 (194).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, long long ldx,
                                                       const int32_t* __restrict__ pair, T* __restrict__ rows, int H,
@@ -204,7 +205,8 @@ __global__ void __launch_bounds__(256) permute_kernel(const T* __restrict__ x, l
 // loads (16 for 8 slots) it issues before it needs one.  The rows' places and
 // weights are read once for all columns.  Bound by memory: 65536 f32 rows of
 // 2816 into 8192 bf16 tokens (785 MB) 120 us, 6.5 TB/s; bf16 rows (415 MB) 70 us,
-// 5.9 TB/s (one vector per thread and CTA: 129 and 75 us).  The weight of slot k is probs[t,k]
+// 5.9 TB/s (one vector per thread and CTA: 129 and 75 us); unaligned rows of
+// 2815, element by element, bf16 315 us, f32 138 (122).  The weight of slot k is probs[t,k]
 // (1 without probs) times scale[ids[t,k]] (with scale).
 template <int TYPE_IN, int TYPE, bool VEC>
 __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE_IN>::T* __restrict__ rows,
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(128) unpermute_kernel(const typename Elem<TYPE
 // A warp per pair: reads the pair's row and the token's gradient once, writes
 // the row's gradient and the weight's.  The K warps of a token share its
 // gradient row through L1.  Bound by memory: 65536 bf16 rows of 2816 (784 MB)
-// 126 us, 6.2 TB/s.  The warp also clears the row of its own index
+// 126 us, 6.2 TB/s; unaligned rows of 2815 218 us, f32 340 (247).  The warp also clears the row of its own index
 // when no pair takes it (there are at least as many rows as pairs).
 template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(256) unpermute_grad_kernel(const typename Elem<TYPE>::T* __restrict__ dout,
